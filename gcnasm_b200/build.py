@@ -12,16 +12,16 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "_lib", "libb2g.so")
-SOURCES = [os.path.join(HERE, "csrc", "b2g_api.cu")]
-# every source and header under csrc/ plus the public header: editing any of them rebuilds
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("b2g_api.cu", "b2g_kv4_api.cu")]
+# every source and header under csrc/ plus the public headers: editing any of them rebuilds
 DEPS = sorted(os.path.join(HERE, "csrc", f) for f in os.listdir(os.path.join(HERE, "csrc"))
-              if f.endswith((".cu", ".cuh", ".h"))) + [os.path.join(ROOT, "include", "b2g", "gemm.h")]
+              if f.endswith((".cu", ".cuh", ".h"))) + [os.path.join(ROOT, "include", "b2g", f)
+                                                       for f in ("gemm.h", "kv4.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-shared",
 ]
 
 
@@ -39,15 +39,36 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(d) <= t for d in DEPS if os.path.exists(d))
 
 
+def _object(src: str) -> str:
+    return os.path.join(HERE, "_lib", os.path.basename(src) + ".o")
+
+
+def _object_up_to_date(src: str) -> bool:
+    """The object is newer than everything its last compilation read (nvcc's dependency file)."""
+    obj = _object(src)
+    if not (os.path.exists(obj) and os.path.exists(obj + ".d")):
+        return False
+    with open(obj + ".d") as f:
+        deps = f.read().replace("\\\n", " ").split(":", 1)[-1].split()
+    t = os.path.getmtime(obj)
+    return src in deps and all(os.path.exists(d) and os.path.getmtime(d) <= t for d in deps)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", os.path.join(HERE, "csrc"),
-           *SOURCES, "-o", LIB + ".tmp"]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
+    todo = []
+    for src in SOURCES:
+        if not force and _object_up_to_date(src):
+            continue
+        obj = _object(src)
+        cmd = [nvcc(), *NVCC_FLAGS, *(["-Xptxas=-v"] if verbose else []), "-I", os.path.join(ROOT, "include"),
+               "-I", os.path.join(HERE, "csrc"), "-MD", "-MF", obj + ".d", "-c", src, "-o", obj]
+        todo.append((cmd, subprocess.Popen(cmd)))
+    for cmd, p in [(c, p) for c, p in todo if p.wait()]:
+        raise subprocess.CalledProcessError(p.returncode, cmd)
+    subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", *map(_object, SOURCES), "-o", LIB + ".tmp"], check=True)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/b2g/gemm.h`` (``_lib/libb2g.so``).
+"""ctypes binding of the C ABI in ``include/b2g/gemm.h`` and ``include/b2g/kv4.h`` (``_lib/libb2g.so``).
 
 The structures mirror the reference's host argument blocks byte for byte:
 
@@ -40,6 +40,11 @@ EXPORTS = [
     "b2g_device_status", "b2g_set_wait_timeout_ms", "b2g_debug_force_stall", "b2g_status_string",
     "b2g_last_error", "b2g_version",
 ]
+
+# every symbol include/b2g/kv4.h declares
+KV4_EXPORTS = ["b2g_kv4_append", "b2g_kv4_read", "b2g_kv4_attention", "b2g_kv4_workspace_bytes", "b2g_kv4_weights",
+               "b2g_kv4_evict"]
+DEV_BAD_PAGE = 5
 
 
 class B2GError(RuntimeError):
@@ -105,6 +110,23 @@ class Epilogue(C.Structure):
     _fields_ = [("c", C.c_void_p), ("ldc", C.c_longlong), ("beta", C.c_float), ("bias", C.c_void_p)]
 
 
+class Kv4Cache(C.Structure):
+    """b2g_kv4_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int), ("head_dim", C.c_int)]
+
+
+class Kv4Batch(C.Structure):
+    """b2g_kv4_batch."""
+    _fields_ = [("table", C.c_void_p), ("lens", C.c_void_p), ("cu", C.c_void_p), ("seqs", C.c_int),
+                ("table_width", C.c_int), ("rows", C.c_int), ("max_new", C.c_int)]
+
+
+class Kv4Mask(C.Structure):
+    """b2g_kv4_mask."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("causal", C.c_int), ("window", C.c_int)]
+
+
 _LIB = None
 
 
@@ -151,6 +173,14 @@ def lib() -> C.CDLL:
         L.b2g_status_string.argtypes = [ci]
         L.b2g_status_string.restype = C.c_char_p
         L.b2g_last_error.restype = C.c_char_p
+        pc, pb, pm = C.POINTER(Kv4Cache), C.POINTER(Kv4Batch), C.POINTER(Kv4Mask)
+        L.b2g_kv4_append.argtypes = [pc, pb, vp, vp, ci, ll, ll, ll, ll, vp, vp]
+        L.b2g_kv4_read.argtypes = [pc, pb, vp, vp, vp, vp]
+        L.b2g_kv4_attention.argtypes = [pc, pb, pm, vp, ll, ll, ci, vp, ll, ll, vp, vp, ll, vp]
+        L.b2g_kv4_workspace_bytes.argtypes = [ci, ci, ci]
+        L.b2g_kv4_workspace_bytes.restype = ll
+        L.b2g_kv4_weights.argtypes = [pc, pb, pm, vp, ll, ll, ci, vp, vp, vp, vp]
+        L.b2g_kv4_evict.argtypes = [pc, pb, vp, ci, ci, ci, vp, ci, vp, vp, vp]
         _LIB = L
     return _LIB
 

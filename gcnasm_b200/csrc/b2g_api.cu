@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "b2g_aux.cuh"
+#include "b2g_host.h"
 #include "b2g_gemm.cuh"
 #include "b2g_gemm_pair.cuh"
 #include "b2g_gemm_skinny.cuh"
@@ -1150,6 +1151,27 @@ int noalloc_env(Env* e) {
 }  // namespace
 
 // =================================================================== C ABI
+namespace b2g {
+
+int host_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int host_device(int* sms, int** status) {
+  DevState* d = nullptr;
+  int rc = device_state(&d);
+  if (rc) return rc;
+  *sms = d->sms;
+  *status = d->status;
+  return B2G_OK;
+}
+
+}  // namespace b2g
+
 extern "C" {
 
 int b2g_version(void) { return kVersion; }

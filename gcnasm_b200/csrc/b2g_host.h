@@ -1,0 +1,13 @@
+// b2g_host.h -- host helpers that the library's translation units share: the error
+// message behind b2g_last_error and the current device's state (b2g_api.cu).
+#pragma once
+
+namespace b2g {
+
+// records the message of b2g_last_error and returns `code`
+int host_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// SM count and device status word of the current device (an sm_100 one); a status code
+int host_device(int* sms, int** status);
+
+}  // namespace b2g

@@ -1,0 +1,219 @@
+// b2g_kv4_api.cu -- C ABI of the 4-bit key/value cache (include/b2g/kv4.h): argument
+// checks and kernel launches.  Nothing here allocates or waits.
+#include "b2g/kv4.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "b2g_host.h"
+#include "b2g_kv4.cuh"
+#include "b2g_kv4_attn.cuh"
+
+using namespace b2g;
+
+namespace {
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B2G_OK : host_fail(B2G_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+}
+
+int grid_for(long long threads, int block, int most) {
+  return static_cast<int>(std::max(1ll, std::min((threads + block - 1) / block, static_cast<long long>(most))));
+}
+
+struct Call {
+  Kv4Cache c;
+  Kv4Batch bt;
+  int dim = 0, sms = 0;
+  int* status = nullptr;
+  cudaStream_t st = nullptr;
+};
+
+// rows: whether the call has rows of its own (cu, rows and max_new count)
+int check(Call* f, const b2g_kv4_cache* c, const b2g_kv4_batch* b, bool lens, bool rows, void* stream) {
+  if (!c || !b) return host_fail(B2G_ERR_INVALID_ARG, "null cache or batch");
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return host_fail(B2G_ERR_INVALID_ARG, "null cache pointer");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
+    return host_fail(B2G_ERR_ALIGNMENT, "cache arrays must be 16-byte aligned");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return host_fail(B2G_ERR_UNSUPPORTED, "head_dim %d is not 64, 128 or 256", c->head_dim);
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    return host_fail(B2G_ERR_UNSUPPORTED, "page_size %d is not a power of two in 16 .. 1024", c->page_size);
+  if (c->kv_heads < 1 || c->kv_heads > 1024) return host_fail(B2G_ERR_UNSUPPORTED, "kv_heads %d is not in 1 .. 1024", c->kv_heads);
+  if (c->pages < 1) return host_fail(B2G_ERR_INVALID_ARG, "pages %d must be positive", c->pages);
+  if (!b->table || (lens && !b->lens)) return host_fail(B2G_ERR_INVALID_ARG, "null page table or lengths");
+  if (b->seqs < 1 || b->seqs > 8192) return host_fail(B2G_ERR_UNSUPPORTED, "seqs %d is not in 1 .. 8192", b->seqs);
+  if (b->table_width < 1 || static_cast<long long>(b->table_width) * c->page_size > 0x7fff0000ll)
+    return host_fail(B2G_ERR_UNSUPPORTED, "table_width %d must be positive and hold less than 2^31 tokens", b->table_width);
+  if (rows) {
+    if (b->rows < 0 || b->max_new < 0) return host_fail(B2G_ERR_INVALID_ARG, "negative row count");
+    if (!b->cu && b->rows != b->seqs)
+      return host_fail(B2G_ERR_INVALID_ARG, "without cu there is one row for each sequence (%d rows, %d sequences)", b->rows, b->seqs);
+  }
+  int rc = host_device(&f->sms, &f->status);
+  if (rc) return rc;
+  f->c.k = static_cast<uint8_t*>(c->k);
+  f->c.v = static_cast<uint8_t*>(c->v);
+  f->c.ks = static_cast<uint8_t*>(c->k_scale);
+  f->c.vs = static_cast<uint8_t*>(c->v_scale);
+  f->c.pages = c->pages;
+  f->c.heads = c->kv_heads;
+  f->c.page_log2 = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  f->bt = Kv4Batch{b->table, b->lens, rows ? b->cu : nullptr, b->seqs, b->table_width, b->rows};
+  f->dim = c->head_dim;
+  f->st = static_cast<cudaStream_t>(stream);
+  return B2G_OK;
+}
+
+int check_queries(const b2g_kv4_cache* c, const b2g_kv4_mask* m, const void* q, long long row, long long head, int heads,
+                  const char* name) {
+  if (!m || !q) return host_fail(B2G_ERR_INVALID_ARG, "null mask or %s", name);
+  if (heads < 1 || heads % c->kv_heads)
+    return host_fail(B2G_ERR_INVALID_ARG, "heads %d must be a positive multiple of kv_heads %d", heads, c->kv_heads);
+  if (!aligned(q, 16) || row % 8 || head % 8 || row < 0 || head < 0)
+    return host_fail(B2G_ERR_ALIGNMENT, "%s needs a 16-byte aligned base and whole 16-byte row and head strides", name);
+  if (!std::isfinite(m->scale) || !std::isfinite(m->softcap) || m->softcap < 0.f || m->window < 0)
+    return host_fail(B2G_ERR_INVALID_ARG, "scale and softcap must be finite, softcap and window not negative");
+  return B2G_OK;
+}
+
+// an empty batch's arrays may be null: there is nothing to do
+inline bool no_rows(const b2g_kv4_batch* b) { return b && b->rows == 0 && b->cu; }
+
+// f(std::integral_constant<int, D>) for the cache's head_dim
+template <typename F>
+void by_dim(int dim, F&& f) {
+  if (dim == 64) f(std::integral_constant<int, 64>());
+  else if (dim == 128) f(std::integral_constant<int, 128>());
+  else f(std::integral_constant<int, 256>());
+}
+
+}  // namespace
+
+extern "C" {
+
+int b2g_kv4_append(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const void* k, const void* v, int x_dtype,
+                   long long k_row_stride, long long k_head_stride, long long v_row_stride, long long v_head_stride,
+                   float* weights, void* stream) {
+  if (x_dtype != B2G_OUT_F32 && x_dtype != B2G_OUT_BF16) return host_fail(B2G_ERR_INVALID_ARG, "x_dtype must be fp32 or bf16");
+  if (no_rows(batch)) return B2G_OK;
+  if (!k || !v) return host_fail(B2G_ERR_INVALID_ARG, "null k or v");
+  const long long e = x_dtype == B2G_OUT_F32 ? 4 : 8;  // elements per 16 bytes
+  for (long long s : {k_row_stride, k_head_stride, v_row_stride, v_head_stride})
+    if (s < 0 || s % e) return host_fail(B2G_ERR_ALIGNMENT, "row and head strides of k and v must be whole 16 bytes");
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(weights, 4))
+    return host_fail(B2G_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
+  Call f;
+  int rc = check(&f, cache, batch, true, true, stream);
+  if (rc) return rc;
+  by_dim(f.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    const int grid = grid_for(static_cast<long long>(batch->rows) * 2 * f.c.heads * (D / 8), 256, 16 * f.sms);
+    if (x_dtype == B2G_OUT_F32)
+      b2g_kv4_append_kernel<float, D><<<grid, 256, 0, f.st>>>(f.c, f.bt, static_cast<const float*>(k), static_cast<const float*>(v),
+                                                              k_row_stride, k_head_stride, v_row_stride, v_head_stride, weights,
+                                                              f.status);
+    else
+      b2g_kv4_append_kernel<__nv_bfloat16, D><<<grid, 256, 0, f.st>>>(
+          f.c, f.bt, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), k_row_stride, k_head_stride,
+          v_row_stride, v_head_stride, weights, f.status);
+  });
+  return launched();
+}
+
+int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const int* start, void* k, void* v, void* stream) {
+  if (no_rows(batch)) return B2G_OK;
+  if (!k || !v || !start) return host_fail(B2G_ERR_INVALID_ARG, "null k, v or start");
+  if (!aligned(k, 16) || !aligned(v, 16)) return host_fail(B2G_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
+  Call f;
+  int rc = check(&f, cache, batch, false, true, stream);
+  if (rc) return rc;
+  by_dim(f.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    const int grid = grid_for(static_cast<long long>(batch->rows) * 2 * f.c.heads * (D / 8), 256, 16 * f.sms);
+    b2g_kv4_read_kernel<D><<<grid, 256, 0, f.st>>>(f.c, f.bt, start, static_cast<__nv_bfloat16*>(k),
+                                                   static_cast<__nv_bfloat16*>(v), f.status);
+  });
+  return launched();
+}
+
+long long b2g_kv4_workspace_bytes(int seqs, int kv_heads, int head_dim) {
+  if (seqs < 1 || kv_heads < 1 || head_dim < 1) return -host_fail(B2G_ERR_INVALID_ARG, "non-positive size");
+  return 16;
+}
+
+int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask, const void* q,
+                      long long q_row_stride, long long q_head_stride, int heads, void* out, long long out_row_stride,
+                      long long out_head_stride, float* lse, void* workspace, long long workspace_bytes, void* stream) {
+  if (no_rows(batch)) return B2G_OK;
+  Call f;
+  int rc = check(&f, cache, batch, true, true, stream);
+  if (rc) return rc;
+  if ((rc = check_queries(cache, mask, q, q_row_stride, q_head_stride, heads, "q"))) return rc;
+  if ((rc = check_queries(cache, mask, out, out_row_stride, out_head_stride, heads, "out"))) return rc;
+  if (!lse || !aligned(lse, 4)) return host_fail(B2G_ERR_INVALID_ARG, "null or misaligned lse");
+  const long long need = b2g_kv4_workspace_bytes(f.bt.seqs, f.c.heads, f.dim);
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+    return host_fail(B2G_ERR_WORKSPACE, "the workspace holds %lld bytes, not %lld (16-byte aligned)", workspace_bytes, need);
+  const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
+  const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
+  by_dim(f.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    b2g_kv4_attention_kernel<D><<<batch->rows * heads, 128, 0, f.st>>>(f.c, f.bt, m, qs, static_cast<__nv_bfloat16*>(out),
+                                                                       out_row_stride, out_head_stride, lse, f.status);
+  });
+  return launched();
+}
+
+int b2g_kv4_weights(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask, const void* q,
+                    long long q_row_stride, long long q_head_stride, int heads, const float* lse, const float* weights_in,
+                    float* weights_out, void* stream) {
+  Call f;
+  int rc = check(&f, cache, batch, true, true, stream);
+  if (rc) return rc;
+  if ((rc = check_queries(cache, mask, q, q_row_stride, q_head_stride, heads, "q"))) return rc;
+  if (!lse || !weights_in || !weights_out || !aligned(lse, 4) || !aligned(weights_in, 4) || !aligned(weights_out, 4))
+    return host_fail(B2G_ERR_INVALID_ARG, "null or misaligned lse or weights");
+  const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
+  const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
+  by_dim(f.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    b2g_kv4_weights_kernel<D><<<dim3(64, f.c.heads, f.bt.seqs), 128, 0, f.st>>>(f.c, f.bt, m, qs, lse, weights_in, weights_out,
+                                                                               f.status);
+  });
+  return launched();
+}
+
+int b2g_kv4_evict(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, float* weights, int budget, int sink, int recent,
+                  const int* out_table, int out_width, int* kept, int* new_lens, void* stream) {
+  Call f;
+  int rc = check(&f, cache, batch, true, false, stream);
+  if (rc) return rc;
+  if (!weights || !out_table || !kept || !new_lens) return host_fail(B2G_ERR_INVALID_ARG, "null weights, out_table, kept or new_lens");
+  if (!aligned(weights, 4) || !aligned(kept, 4)) return host_fail(B2G_ERR_ALIGNMENT, "misaligned weights or kept");
+  if (budget < 1 || sink < 0 || recent < 0 || static_cast<long long>(sink) + recent > budget)
+    return host_fail(B2G_ERR_INVALID_ARG, "budget must be positive and hold sink and recent");
+  const bool in_place = out_table == batch->table;
+  if (out_width < 1 || (in_place && out_width != batch->table_width) ||
+      static_cast<long long>(out_width) * cache->page_size < std::min<long long>(budget, static_cast<long long>(batch->table_width) * cache->page_size))
+    return host_fail(B2G_ERR_INVALID_ARG, "out_table of %d pages a sequence does not hold the budget of %d tokens", out_width, budget);
+  const int lists = f.bt.seqs * f.c.heads;
+  b2g_kv4_select_kernel<<<lists, kEvictThreads, 0, f.st>>>(f.c, f.bt, weights, budget, sink, recent, kept, f.status);
+  if ((rc = launched())) return rc;
+  by_dim(f.dim, [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (in_place)
+      b2g_kv4_move_in_place_kernel<D><<<lists, 1024, 0, f.st>>>(f.c, f.bt, weights, budget, kept, new_lens, f.status);
+    else
+      b2g_kv4_move_kernel<D><<<grid_for(static_cast<long long>(lists) * budget * (D / 16 + 1), 256, 16 * f.sms), 256, 0, f.st>>>(
+          f.c, f.bt, weights, budget, out_table, out_width, kept, new_lens, f.status);
+  });
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,214 @@
+"""The 4-bit key/value cache and the attention over it, for torch tensors.
+
+K and V are held as MXFP4 -- packed E2M1 codes (element 2i in the low nibble) and one UE8M0
+scale byte per 32 channels, the formats of :func:`ops.mxfp4_gemm`'s operands -- in pages of
+``page_size`` tokens.  Sequence ``b``'s token ``j`` lies in page ``table[b, j // page_size]``,
+slot ``j % page_size``; ``lens[b]`` counts its cached tokens, this step's among them.  The rows
+``cu[b]:cu[b + 1]`` of q, k and v are its last tokens, in order; without ``cu`` each sequence
+has one row.  ``table``, ``lens`` and ``cu`` are int32 on the GPU, so that a decode loop never
+waits for it; ``max_new`` / ``max_q`` tell the host how many rows a sequence has at most.
+
+PyTorch supplies memory and streams; the computation runs in ``libb2g.so``
+(``include/b2g/kv4.h`` has the exact semantics).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import capi
+from .ops import _stream
+
+HEAD_DIMS = (64, 128, 256)
+
+
+class KV4Cache:
+    """The arrays of one cache: uint8 k, v ``[pages, kv_heads, page_size, head_dim / 2]`` and
+    k_scale, v_scale ``[pages, kv_heads, page_size, head_dim / 32]``, contiguous."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "_args")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        shape, sf = k.shape, k_scale.shape
+        if k.dim() != 4 or v.shape != shape or v_scale.shape != sf or sf[:3] != shape[:3] or sf[3] * 16 != shape[3]:
+            raise ValueError("k, v: [pages, kv_heads, page_size, head_dim / 2]; scales: [..., head_dim / 32]")
+        for t in (k, v, k_scale, v_scale):
+            if t.dtype is not torch.uint8 or not t.is_contiguous() or not t.is_cuda:
+                raise ValueError("cache arrays must be contiguous uint8 CUDA tensors")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.kv_heads, self.page_size, self.head_dim = shape[0], shape[1], shape[2], 2 * shape[3]
+        self._args = capi.Kv4Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], shape[1],
+                                   shape[2], 2 * shape[3])
+
+
+def alloc(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> KV4Cache:
+    """An empty cache (every value zero)."""
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
+
+    def zeros(width):
+        return torch.zeros((pages, kv_heads, page_size, width), dtype=torch.uint8, device=device)
+
+    return KV4Cache(zeros(head_dim // 2), zeros(head_dim // 2), zeros(head_dim // 32), zeros(head_dim // 32))
+
+
+def alloc_weights(cache: KV4Cache) -> torch.Tensor:
+    """fp32 ``[pages, kv_heads, page_size]`` for the attention weight each cached token gathers."""
+    return torch.zeros((cache.pages, cache.kv_heads, cache.page_size), dtype=torch.float32, device=cache.k.device)
+
+
+def _ints(t: torch.Tensor, name: str, dim: int, size: int | None = None) -> int:
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous() or t.dim() != dim:
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of {dim} dimension(s)")
+    if size is not None and t.shape[0] != size:
+        raise ValueError(f"{name} has {t.shape[0]} entries, not {size}")
+    return t.data_ptr()
+
+
+def _batch(table, lens, cu, rows: int, max_new: int | None) -> capi.Kv4Batch:
+    tp = _ints(table, "table", 2)
+    seqs, width = table.shape
+    lp = _ints(lens, "lens", 1, seqs) if lens is not None else None
+    cp = _ints(cu, "cu", 1, seqs + 1) if cu is not None else None
+    if max_new is None:
+        max_new = rows if cu is not None else 1
+    return capi.Kv4Batch(tp, lp, cp, seqs, width, rows, max_new)
+
+
+def _heads(t: torch.Tensor, name: str, cache: KV4Cache) -> None:
+    if t.dim() != 3 or not t.is_cuda or t.shape[2] != cache.head_dim or t.stride(2) != 1:
+        raise ValueError(f"{name} must be a CUDA tensor [rows, heads, {cache.head_dim}] with unit channel stride")
+
+
+def _weights_array(t: torch.Tensor, name: str, cache: KV4Cache) -> int:
+    if t.dtype is not torch.float32 or not t.is_cuda or not t.is_contiguous() or \
+            t.shape != (cache.pages, cache.kv_heads, cache.page_size):
+        raise ValueError(f"{name} must be a contiguous fp32 CUDA tensor [pages, kv_heads, page_size]")
+    return t.data_ptr()
+
+
+def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+           cu: torch.Tensor | None = None, max_new: int | None = None, weights: torch.Tensor | None = None,
+           stream=None) -> None:
+    """Quantises k, v (bf16 or fp32 ``[rows, kv_heads, head_dim]``, any row and head strides of whole
+    16 bytes) into the cache as the sequences' last tokens.  ``weights``: its entries of the new tokens
+    become zero."""
+    _heads(k, "k", cache)
+    _heads(v, "v", cache)
+    if v.dtype is not k.dtype or v.shape != k.shape or k.shape[1] != cache.kv_heads:
+        raise ValueError("k and v must have one dtype and shape [rows, kv_heads, head_dim]")
+    if k.dtype is torch.bfloat16:
+        code = capi.OUT_BF16
+    elif k.dtype is torch.float32:
+        code = capi.OUT_F32
+    else:
+        raise ValueError(f"k and v must be fp32 or bf16, not {k.dtype}")
+    b = _batch(table, lens, cu, k.shape[0], max_new)
+    wp = _weights_array(weights, "weights", cache) if weights is not None else None
+    capi.check(capi.lib().b2g_kv4_append(cache._args, b, k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1),
+                                         v.stride(0), v.stride(1), wp, _stream(stream)), "b2g_kv4_append")
+
+
+def read(cache: KV4Cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor | None, rows: int,
+         stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 (k, v) ``[rows, kv_heads, head_dim]``: rows ``cu[b]:cu[b + 1]`` hold sequence b's tokens
+    ``start[b]``, ``start[b] + 1``, ... as the cache has them."""
+    b = _batch(table, None, cu, rows, None)
+    sp = _ints(start, "start", 1, b.seqs)
+    out = torch.empty((2, rows, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.k.device)
+    k, v = out.unbind(0)
+    capi.check(capi.lib().b2g_kv4_read(cache._args, b, sp, k.data_ptr(), v.data_ptr(), _stream(stream)), "b2g_kv4_read")
+    return k, v
+
+
+_WORKSPACES: dict = {}
+
+
+def workspace(cache: KV4Cache, seqs: int) -> torch.Tensor:
+    """A zeroed workspace for :func:`attention` calls of up to ``seqs`` sequences: calls that may overlap
+    on the GPU need one each."""
+    n = int(capi.lib().b2g_kv4_workspace_bytes(seqs, cache.kv_heads, cache.head_dim))
+    if n < 0:
+        capi.check(-n, "b2g_kv4_workspace_bytes")
+    return torch.zeros(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def _workspace(cache: KV4Cache, seqs: int, stream: int | None) -> torch.Tensor:
+    """The workspace this module keeps for a device and stream, grown where it is too small."""
+    key = (cache.k.device.index, stream, cache.kv_heads, cache.head_dim)
+    held = _WORKSPACES.get(key)
+    if held is None or held[0] < seqs:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream or 0, device=cache.k.device)):  # zeroed in that stream's order
+            held = _WORKSPACES[key] = (seqs, workspace(cache, seqs))
+    return held[1]
+
+
+def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor | None = None,
+              max_q: int | None = None, scale: float | None = None, causal: bool = True, window: int = 0,
+              softcap: float = 0.0, out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+              stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse): bf16 q ``[rows, heads, head_dim]`` attends over what is cached (``heads`` a multiple of
+    the cache's kv_heads).  The query of the token at position p sees token j < lens[b] when j <= p
+    (``causal``) and j > p - window (``window`` > 0); scores are ``scale * q . k`` (default
+    head_dim ** -0.5), capped as ``softcap * tanh(s / softcap)``.  lse fp32 ``[rows, heads]`` is the
+    logarithm of the sum of exp(scores); a query that sees nothing gives out 0 and lse -inf."""
+    _heads(q, "q", cache)
+    if q.dtype is not torch.bfloat16:
+        raise ValueError(f"q must be bf16, not {q.dtype}")
+    rows, heads = q.shape[0], q.shape[1]
+    b = _batch(table, lens, cu, rows, max_q)
+    if out is None:
+        out = torch.empty((rows, heads, cache.head_dim), dtype=torch.bfloat16, device=q.device)
+    else:
+        _heads(out, "out", cache)
+        if out.dtype is not torch.bfloat16 or out.shape != q.shape:
+            raise ValueError("out must be bf16 of q's shape")
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device)
+    st = _stream(stream)
+    if ws is None:
+        ws = _workspace(cache, b.seqs, st.value)
+    mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
+    capi.check(capi.lib().b2g_kv4_attention(cache._args, b, mask, q.data_ptr(), q.stride(0), q.stride(1), heads,
+                                            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), ws.data_ptr(),
+                                            ws.numel(), st), "b2g_kv4_attention")
+    return out, lse
+
+
+def weights(q: torch.Tensor, lse: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor,
+            gathered: torch.Tensor, cu: torch.Tensor | None = None, max_q: int | None = None, scale: float | None = None,
+            causal: bool = True, window: int = 0, softcap: float = 0.0, out: torch.Tensor | None = None,
+            stream=None) -> torch.Tensor:
+    """``gathered`` (fp32 ``[pages, kv_heads, page_size]``) plus, for each cached token of the batch, the
+    attention weight exp(score - lse) summed over the sequence's query rows and the kv head's query heads;
+    written to ``out`` (default: ``gathered`` itself).  q, lse and the mask as for :func:`attention`."""
+    _heads(q, "q", cache)
+    if q.dtype is not torch.bfloat16:
+        raise ValueError(f"q must be bf16, not {q.dtype}")
+    if lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2] or not lse.is_cuda:
+        raise ValueError("lse must be a contiguous fp32 CUDA tensor [rows, heads]")
+    out = gathered if out is None else out
+    b = _batch(table, lens, cu, q.shape[0], max_q)
+    mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
+    capi.check(capi.lib().b2g_kv4_weights(cache._args, b, mask, q.data_ptr(), q.stride(0), q.stride(1), q.shape[1],
+                                          lse.data_ptr(), _weights_array(gathered, "gathered", cache),
+                                          _weights_array(out, "out", cache), _stream(stream)), "b2g_kv4_weights")
+    return out
+
+
+def evict(cache: KV4Cache, gathered: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, budget: int, sink: int = 4,
+          recent: int = 64, out_table: torch.Tensor | None = None, out_lens: torch.Tensor | None = None,
+          stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(kept, new lens): thins each sequence out to ``budget`` tokens, each kv head by itself -- the first
+    ``sink``, the last ``recent`` and the heaviest of the others by ``gathered``, in their order.  They move
+    to the pages of ``out_table`` (default: in place, to the first pages of ``table``), their gathered
+    weights with them.  kept: int32 ``[seqs, kv_heads, budget]``, the numbers they had, then -1;
+    ``out_lens`` may be ``lens``."""
+    b = _batch(table, lens, None, table.shape[0], None)
+    out_table = table if out_table is None else out_table
+    op = _ints(out_table, "out_table", 2, b.seqs)
+    if out_lens is None:
+        out_lens = torch.empty_like(lens)
+    kept = torch.empty((b.seqs, cache.kv_heads, max(budget, 0)), dtype=torch.int32, device=lens.device)
+    capi.check(capi.lib().b2g_kv4_evict(cache._args, b, _weights_array(gathered, "gathered", cache), budget, sink, recent, op,
+                                        out_table.shape[1], kept.data_ptr(), _ints(out_lens, "out_lens", 1, b.seqs),
+                                        _stream(stream)), "b2g_kv4_evict")
+    return kept, out_lens

@@ -1,0 +1,133 @@
+/*
+ * b2g/kv4.h -- C ABI of the 4-bit key/value cache and the attention over it.
+ *
+ * The cache holds K and V as MXFP4, the element and scale formats of b2g_gemm_mxfp4's
+ * operands: packed E2M1 codes (element 2i in the low nibble) and one UE8M0 scale byte
+ * (2^(byte - 127)) per 32 channels, 4.25 bits per value.  Tokens lie in pages of
+ * page_size tokens; sequence b's token j lies in page table[b * table_width + j / page_size],
+ * slot j % page_size.  The conventions of b2g/gemm.h hold: plain pointers to device
+ * memory, an opaque stream handle (a cudaStream_t, NULL = legacy default stream), every
+ * call stream-ordered and returning a status code, b2g_last_error() for the message.
+ * No call allocates or waits, so all of them can be captured in a CUDA graph once a
+ * first call has been made on the device.
+ *
+ * Sizes that the device holds (lens, cu, page numbers) are not known to the host, so
+ * the kernels bound them: a length is cut to the table's capacity, a row range to the
+ * rows given, and a page number outside [0, pages) makes its tokens absent (not written,
+ * not attended to, read as zeros) and sets the device status word to B2G_DEV_BAD_PAGE
+ * (b2g_device_status).
+ */
+#ifndef B2G_KV4_H
+#define B2G_KV4_H
+
+#include "b2g/gemm.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* device status word (b2g_device_status): a page table named a page that is not there */
+enum { B2G_DEV_BAD_PAGE = 5 };
+
+/* Scale bytes the cache holds: 2^-60 .. 2^65.  b2g_kv4_append clamps to them (larger
+ * magnitudes saturate at 6 * 2^65, smaller ones round to zero), the readers clamp what
+ * they find, so that products with a scale stay normal bf16 and fp32 numbers. */
+enum { B2G_KV4_SCALE_MIN = 67, B2G_KV4_SCALE_MAX = 192 };
+
+/* k, v:             [pages][kv_heads][page_size][head_dim / 2] bytes
+ * k_scale, v_scale: [pages][kv_heads][page_size][head_dim / 32] bytes
+ * contiguous, 16-byte aligned.  head_dim 64, 128 or 256; page_size a power of two in
+ * 16 .. 1024; kv_heads 1 .. 1024. */
+typedef struct b2g_kv4_cache {
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    int pages;
+    int kv_heads;
+    int page_size;
+    int head_dim;
+} b2g_kv4_cache;
+
+/* The sequences of one call.  lens[b] counts sequence b's cached tokens, this step's
+ * among them; its rows of q / k / v are cu[b] .. cu[b + 1] - 1 (cu[0] = 0, ascending)
+ * and stand for its last tokens, in order.  cu = NULL: one row for each sequence
+ * (rows = seqs).  max_new: an upper bound of a sequence's rows (host side).
+ * seqs 1 .. 8192. */
+typedef struct b2g_kv4_batch {
+    const int* table; /* [seqs][table_width] page numbers */
+    const int* lens;  /* [seqs] */
+    const int* cu;    /* [seqs + 1] or NULL */
+    int seqs;
+    int table_width;
+    int rows;
+    int max_new;
+} b2g_kv4_batch;
+
+/* Scores s = scale * q . k; softcap > 0: s = softcap * tanh(s / softcap).  The query at
+ * position p (its own token's index) sees token j when j < length, j <= p (causal != 0)
+ * and j > p - window (window > 0). */
+typedef struct b2g_kv4_mask {
+    float scale;
+    float softcap;
+    int causal;
+    int window;
+} b2g_kv4_mask;
+
+/* Quantises rows of K and V into the cache (the MXFP4 quantiser's rule, b2g_quant_mxfp4:
+ * per 32 channels the least power of two s with 6 s >= amax, nearest code of x / s, a
+ * tie to the even code; a NaN becomes 6 s).  k, v: element (row, head, channel) at row * *_row_stride +
+ * head * *_head_stride + channel, of x_dtype (B2G_OUT_BF16 / B2G_OUT_F32); bases and
+ * strides whole 16 bytes.  weights (may be NULL): fp32 [pages][kv_heads][page_size]; the
+ * appended tokens' entries become zero. */
+B2G_API int b2g_kv4_append(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const void* k, const void* v,
+                           int x_dtype, long long k_row_stride, long long k_head_stride, long long v_row_stride,
+                           long long v_head_stride, float* weights, void* stream);
+
+/* Dequantises tokens start[b] + i (i = 0 .. cu[b + 1] - cu[b] - 1) of each sequence into
+ * row cu[b] + i of k and v: bf16 [rows][kv_heads][head_dim], contiguous, 16-byte aligned.
+ * lens is not used. */
+B2G_API int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const int* start, void* k, void* v,
+                         void* stream);
+
+/* out = softmax(scores) V over what is cached, per query row and head (kv head =
+ * head / (heads / kv_heads)); lse = ln of the sum of exp(scores), fp32 [rows][heads]
+ * contiguous.  A query that sees no token gives out = 0, lse = -inf.  q, out: bf16,
+ * element (row, head, channel) at row * *_row_stride + head * *_head_stride + channel,
+ * bases and strides whole 16 bytes.  heads a multiple of kv_heads.
+ * workspace: b2g_kv4_workspace_bytes(...) bytes, 16-byte aligned, zeroed once by the
+ * caller before its first use; each call leaves it ready for the next.  Calls that
+ * overlap on the GPU need a workspace each. */
+B2G_API int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask,
+                              const void* q, long long q_row_stride, long long q_head_stride, int heads, void* out,
+                              long long out_row_stride, long long out_head_stride, float* lse, void* workspace,
+                              long long workspace_bytes, void* stream);
+
+/* Upper bound, over all lengths, of b2g_kv4_attention's workspace on the current device;
+ * negative: a status code. */
+B2G_API long long b2g_kv4_workspace_bytes(int seqs, int kv_heads, int head_dim);
+
+/* Attention weight gathered by each cached token: weights_out = weights_in + sum over the
+ * sequence's query rows and the kv head's query heads of exp(score - lse), for every
+ * cached token of the batch's sequences (zero is added where no query sees it); lse as
+ * b2g_kv4_attention gives it.  weights_*: fp32 [pages][kv_heads][page_size], which may be
+ * one array; the sequences' pages must be distinct. */
+B2G_API int b2g_kv4_weights(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask,
+                            const void* q, long long q_row_stride, long long q_head_stride, int heads,
+                            const float* lse, const float* weights_in, float* weights_out, void* stream);
+
+/* Thins each sequence out to at most `budget` tokens, separately for each kv head: the
+ * first `sink`, the last `recent`, and of the others those of the largest weight (of
+ * equal ones the earlier; NaN ranks below all), kept in their order.  The kept tokens'
+ * K, V, scales and weights move to tokens 0, 1, ... of the pages in out_table
+ * [seqs][out_width] (out_width * page_size >= budget), either the pages of `table` itself
+ * (out_table == table: in place) or pages that none of these sequences uses.
+ * kept: int32 [seqs][kv_heads][budget], the token numbers, then -1; new_lens [seqs] =
+ * min(length, budget), may be lens itself.  batch->cu, rows and max_new are not used. */
+B2G_API int b2g_kv4_evict(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, float* weights, int budget, int sink,
+                          int recent, const int* out_table, int out_width, int* kept, int* new_lens, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* B2G_KV4_H */
