@@ -177,7 +177,7 @@ def lib() -> C.CDLL:
         L.b2g_kv4_append.argtypes = [pc, pb, vp, vp, ci, ll, ll, ll, ll, vp, vp]
         L.b2g_kv4_read.argtypes = [pc, pb, vp, vp, vp, vp]
         L.b2g_kv4_attention.argtypes = [pc, pb, pm, vp, ll, ll, ci, vp, ll, ll, vp, vp, ll, vp]
-        L.b2g_kv4_workspace_bytes.argtypes = [ci, ci, ci]
+        L.b2g_kv4_workspace_bytes.argtypes = [ci]
         L.b2g_kv4_workspace_bytes.restype = ll
         L.b2g_kv4_weights.argtypes = [pc, pb, pm, vp, ll, ll, ci, vp, vp, vp, vp]
         L.b2g_kv4_evict.argtypes = [pc, pb, vp, ci, ci, ci, vp, ci, vp, vp, vp]

@@ -1161,9 +1161,9 @@ int host_fail(int code, const char* fmt, ...) {
   return code;
 }
 
-int host_device(int* sms, int** status) {
+int host_device(int* sms, int** status, int* dev) {
   DevState* d = nullptr;
-  int rc = device_state(&d);
+  int rc = device_state(&d, dev);
   if (rc) return rc;
   *sms = d->sms;
   *status = d->status;

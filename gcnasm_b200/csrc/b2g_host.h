@@ -7,7 +7,7 @@ namespace b2g {
 // records the message of b2g_last_error and returns `code`
 int host_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
-// SM count and device status word of the current device (an sm_100 one); a status code
-int host_device(int* sms, int** status);
+// SM count, status word and number (0 .. 63) of the current device (an sm_100 one); a status code
+int host_device(int* sms, int** status, int* dev = nullptr);
 
 }  // namespace b2g

@@ -5,11 +5,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "b2g_host.h"
 #include "b2g_kv4.cuh"
-#include "b2g_kv4_attn.cuh"
+#include "b2g_kv4_decode.cuh"
+#include "b2g_kv4_weights.cuh"
 
 using namespace b2g;
 
@@ -29,7 +31,7 @@ int grid_for(long long threads, int block, int most) {
 struct Call {
   Kv4Cache c;
   Kv4Batch bt;
-  int dim = 0, sms = 0;
+  int dim = 0, sms = 0, dev = 0;
   int* status = nullptr;
   cudaStream_t st = nullptr;
 };
@@ -55,7 +57,7 @@ int check(Call* f, const b2g_kv4_cache* c, const b2g_kv4_batch* b, bool lens, bo
     if (!b->cu && b->rows != b->seqs)
       return host_fail(B2G_ERR_INVALID_ARG, "without cu there is one row for each sequence (%d rows, %d sequences)", b->rows, b->seqs);
   }
-  int rc = host_device(&f->sms, &f->status);
+  int rc = host_device(&f->sms, &f->status, &f->dev);
   if (rc) return rc;
   f->c.k = static_cast<uint8_t*>(c->k);
   f->c.v = static_cast<uint8_t*>(c->v);
@@ -77,6 +79,7 @@ int check_queries(const b2g_kv4_cache* c, const b2g_kv4_mask* m, const void* q, 
     return host_fail(B2G_ERR_INVALID_ARG, "heads %d must be a positive multiple of kv_heads %d", heads, c->kv_heads);
   if (!aligned(q, 16) || row % 8 || head % 8 || row < 0 || head < 0)
     return host_fail(B2G_ERR_ALIGNMENT, "%s needs a 16-byte aligned base and whole 16-byte row and head strides", name);
+  if (std::fabs(m->scale) > 0x1p60f) return host_fail(B2G_ERR_INVALID_ARG, "scale beyond 2^60");
   if (!std::isfinite(m->scale) || !std::isfinite(m->softcap) || m->softcap < 0.f || m->window < 0)
     return host_fail(B2G_ERR_INVALID_ARG, "scale and softcap must be finite, softcap and window not negative");
   return B2G_OK;
@@ -91,6 +94,68 @@ void by_dim(int dim, F&& f) {
   if (dim == 64) f(std::integral_constant<int, 64>());
   else if (dim == 128) f(std::integral_constant<int, 128>());
   else f(std::integral_constant<int, 256>());
+}
+
+// A launch that may begin while the kernel before it ends (each kernel waits for that one first).
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? B2G_OK : host_fail(B2G_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+}
+
+// CTAs of a decode kernel on an SM at most, which the workspace is sized for
+constexpr int decode_ctas(int nt) { return nt == 1 ? 4 : 2; }
+
+long long decode_workspace(int sms, int dim) {
+  long long most = 0;
+  for (int nt : {1, 2, 4}) {
+    const long long ctas = static_cast<long long>(sms) * decode_ctas(nt);
+    most = std::max(most, ctas * 16 + 2 * ctas * 8 * nt * (dim + 2) * 4);
+  }
+  return most;
+}
+
+// Resident CTAs per SM, at most `most`, of a kernel with `smem` dynamic bytes on the current
+// device; 0: it does not fit.  Asked of the runtime once per kernel, device and size class.
+template <typename K>
+int resident(K kernel, int block, size_t smem, int most, int dev, std::atomic<int> (&known)[64]) {
+  int n = known[dev].load();
+  if (n) return n;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  n = std::min(n, most);
+  known[dev].store(n);
+  return n;
+}
+
+template <int D, int NT>
+int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, void* workspace) {
+  using Cfg = DecodeCfg<D, NT>;
+  static std::atomic<int> few[64], many[64];
+  // room for the prefix sums of 512 sequences, or of as many as there can be
+  const bool is_few = f.bt.seqs <= 512;
+  const size_t smem = ((Cfg::kFixed + 15) & ~15) + ((is_few ? 512 : 8192) + 1) * sizeof(long long);
+  const int n = resident(b2g_kv4_decode_kernel<D, NT>, 128, smem, decode_ctas(NT), f.dev, is_few ? few : many);
+  if (n < 1) return host_fail(B2G_ERR_CUDA, "the decode kernel does not fit on the device");
+  const int grid = n * f.sms;
+  int4* desc = static_cast<int4*>(workspace);
+  float* partial = reinterpret_cast<float*>(desc + grid);
+  int rc = launch(b2g_kv4_decode_kernel<D, NT>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
+  if (rc) return rc;
+  return launch(b2g_kv4_join_kernel<D, NT>, dim3(grid), 512, 0, f.st, f.c, f.bt, q, o, partial, desc);
 }
 
 }  // namespace
@@ -142,9 +207,12 @@ int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const i
   return launched();
 }
 
-long long b2g_kv4_workspace_bytes(int seqs, int kv_heads, int head_dim) {
-  if (seqs < 1 || kv_heads < 1 || head_dim < 1) return -host_fail(B2G_ERR_INVALID_ARG, "non-positive size");
-  return 16;
+long long b2g_kv4_workspace_bytes(int head_dim) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return -host_fail(B2G_ERR_UNSUPPORTED, "head_dim %d is not 64, 128 or 256", head_dim);
+  int sms = 0, *status = nullptr;
+  const int rc = host_device(&sms, &status);
+  return rc ? -rc : decode_workspace(sms, head_dim);
 }
 
 int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask, const void* q,
@@ -157,17 +225,20 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   if ((rc = check_queries(cache, mask, q, q_row_stride, q_head_stride, heads, "q"))) return rc;
   if ((rc = check_queries(cache, mask, out, out_row_stride, out_head_stride, heads, "out"))) return rc;
   if (!lse || !aligned(lse, 4)) return host_fail(B2G_ERR_INVALID_ARG, "null or misaligned lse");
-  const long long need = b2g_kv4_workspace_bytes(f.bt.seqs, f.c.heads, f.dim);
+  const long long need = decode_workspace(f.sms, f.dim);
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
     return host_fail(B2G_ERR_WORKSPACE, "the workspace holds %lld bytes, not %lld (16-byte aligned)", workspace_bytes, need);
   const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
+  const Kv4Out o{static_cast<__nv_bfloat16*>(out), out_row_stride, out_head_stride, lse};
+  const long long rows = static_cast<long long>(std::max(1, batch->cu ? batch->max_new : 1)) * qs.group;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    b2g_kv4_attention_kernel<D><<<batch->rows * heads, 128, 0, f.st>>>(f.c, f.bt, m, qs, static_cast<__nv_bfloat16*>(out),
-                                                                       out_row_stride, out_head_stride, lse, f.status);
+    if (rows <= 8) rc = decode<D, 1>(f, m, qs, o, workspace);
+    else if (rows <= 16 || D == 256) rc = decode<D, 2>(f, m, qs, o, workspace);
+    else if constexpr (D < 256) rc = decode<D, 4>(f, m, qs, o, workspace);
   });
-  return launched();
+  return rc;
 }
 
 int b2g_kv4_weights(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask, const void* q,

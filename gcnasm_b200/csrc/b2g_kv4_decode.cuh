@@ -1,0 +1,701 @@
+// b2g_kv4_decode.cuh -- attention of few query rows over the 4-bit cache.
+//
+// For one kv head and up to 8 NT query rows (query tokens x heads of the group):
+//   S^T = K Q^T      16 tokens x 8 rows x 16 channels per mma.sync (bf16, fp32 sums)
+//   P = 2^(S - m), m the running maximum, l the running sum (fp32)
+//   O^T += V^T P^T   16 channels x 8 rows x 16 tokens per mma.sync
+//
+// What bounds it: the cache's bytes (D + D / 16 per token and kv head).  At 6.5 TB/s an SM
+// gets ~43 codes a clock, so the codes have to become bf16 in about two integer operations
+// each; there is no time for more.  E2M1's s ee m is placed at a bf16's sign, low exponent
+// bits and top mantissa bit -- the value times 2^-126, a subnormal where e = 0 -- with shifts
+// and masks on two codes at once, and one packed multiplication by 2^(scale + 126 - 64) makes
+// it K or V times 2^-64: exact, since the scale's range is cut to 2^-60 .. 2^65.  The two
+// factors 2^64 go into the score scale and the final division.  Tensor cores here are the
+// warp-level ones: the rows of a decode step fill a sixteenth of a tcgen05 tile, and
+// its operands would have to pass through shared memory once more.
+//
+// Tokens are dealt to warps 32 at a time: each warp keeps m, l and O for its own tokens, fed by
+// its own ring of cp.async stages, and meets the others only at the end of a piece.  Work is
+// cut evenly: the (sequence, kv head, row block) items, laid end to end in units of 128
+// tokens, are divided among as many CTAs as fit on the GPU.  An item cut across CTAs leaves
+// partial results that a second kernel joins in a fixed order.
+#pragma once
+
+#include "b2g_kv4.cuh"
+
+namespace b2g {
+
+struct Kv4Mask {
+  float scale, softcap;
+  int causal, window;
+};
+
+struct Kv4Queries {
+  const __nv_bfloat16* q;
+  long long q_row, q_head;
+  int heads, group;
+};
+
+struct Kv4Out {
+  __nv_bfloat16* out;
+  long long row, head;
+  float* lse;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kTwo64 = 18446744073709551616.f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// c tanh(s / c).  Small arguments by the odd series (to x^11: 6e-8 relative at 0.4), where
+// 1 - 2 / (e^2x + 1) would cancel; that form for the rest has exact limits at both ends.
+__device__ __forceinline__ float kv4_cap(float s, float cap, float two_log2e_over_cap) {
+  const float x = s * two_log2e_over_cap * (0.5f * kLn2), y = x * x;
+  float p = fmaf(y, -1382.f / 155925.f, 62.f / 2835.f);
+  p = fmaf(y, p, -17.f / 315.f);
+  p = fmaf(y, p, 2.f / 15.f);
+  p = fmaf(y, p, -1.f / 3.f);
+  p = fmaf(x * y, p, x);
+  const float far = 1.f - __fdividef(2.f, ex2(s * two_log2e_over_cap) + 1.f);
+  return cap * (fabsf(x) < 0.4f ? p : far);
+}
+
+// Tokens [lo, hi) that the query at position p of a sequence of `len` tokens sees.
+__device__ __forceinline__ void kv4_visible(const Kv4Mask& m, int p, int len, int& lo, int& hi) {
+  hi = m.causal ? min(max(p + 1, 0), len) : len;
+  lo = m.window > 0 ? max(p - m.window + 1, 0) : 0;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma_bf16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Codes I and I + 4 of a word, as bf16 values times 2^-126 (low and high half).
+template <int I>
+__device__ __forceinline__ uint32_t kv4_raw(uint32_t w) {
+  static_assert(I >= 0 && I < 4, "four codes in each half");
+  const uint32_t sign = I == 3 ? w : w << (12 - 4 * I);
+  const uint32_t mag = I < 2 ? w << (6 - 4 * I) : w >> (4 * I - 6);
+  return (sign & 0x80008000u) | (mag & 0x01C001C0u);
+}
+
+// 2^(scale + 126 - 64) as a bf16, for a scale byte cut to the cache's range.
+__device__ __forceinline__ uint32_t kv4_scale_bf16(uint32_t byte) {
+  return (min(max(byte, static_cast<uint32_t>(kKv4ScaleMin)), static_cast<uint32_t>(kKv4ScaleMax)) + 62u) << 7;
+}
+
+// ---------------------------------------------------------------------------
+// work: items (sequence, kv head, row block) in units of kUnit tokens
+// ---------------------------------------------------------------------------
+constexpr int kUnit = 128;
+
+// What a sequence's rows see of its tokens, and how many units that is.
+struct Kv4Span {
+  int first, rows;  // rows of q
+  int len;
+  int base, units;  // first token (a multiple of 16) and units of an item
+};
+
+__device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& bt, const Kv4Mask& m, int b, int page_log2) {
+  Kv4Span s;
+  int end;
+  kv4_rows(bt, b, s.first, end);
+  s.rows = end - s.first;
+  s.len = kv4_len(bt, b, page_log2);
+  int lo, hi, unused;
+  kv4_visible(m, s.len - s.rows, s.len, lo, unused);  // the first row sees furthest back
+  kv4_visible(m, s.len - 1, s.len, unused, hi);
+  s.base = min(lo, hi) & ~15;
+  s.units = s.rows ? max(1, (hi - s.base + kUnit - 1) / kUnit) : 0;
+  return s;
+}
+
+template <int D, int NT>
+struct DecodeCfg {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kChunks = D / 32;              // 16-byte pieces of a token's K (or V), and its scales
+  static constexpr int kHalf = 32 * (D / 2);          // bytes of 32 tokens' K
+  static constexpr int kStage = 2 * kHalf + 64 * kChunks;
+  // bytes in flight on an SM are CTAs x 4 warps x (stages - 1) x kStage
+  static constexpr int kStages = NT == 1 ? (D == 256 ? 3 : D == 128 ? 4 : 6) : (D == 256 ? 2 : D == 128 ? 3 : 5);
+  static constexpr int kMergeStride = D + 4;          // fp32 row of a warp's O: rows 2t of four t in distinct banks
+  static constexpr int kMerge = 4 * kRows * kMergeStride * 4;
+  static constexpr int kQ = (D / 16) * NT * 256;      // Q as B fragments
+  static constexpr int kFixed = 4 * kStages * kStage + kMerge + kQ + 2 * 4 * kRows * 4 + 4 * kStages * 4;
+};
+
+// Position of an item's units among all, walked unit by unit.
+struct Kv4Walk {
+  int b, h, rb, chunk;
+  Kv4Span s;
+  int blocks;  // row blocks of the sequence
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(128)
+b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, float* __restrict__ partial,
+                      int4* __restrict__ desc, int* status) {
+  using Cfg = DecodeCfg<D, NT>;
+  constexpr int kRows = Cfg::kRows, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
+  constexpr int kMT = D / 16;  // 16-channel tiles of O
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * kStages * Cfg::kStage;
+  float* s_merge = reinterpret_cast<float*>(smem + 4 * kStages * Cfg::kStage);
+  uint2* s_q = reinterpret_cast<uint2*>(s_merge + Cfg::kMerge / 4);
+  float* s_m = reinterpret_cast<float*>(s_q + Cfg::kQ / 8);  // [4][kRows]
+  float* s_l = s_m + 4 * kRows;
+  int* s_there = reinterpret_cast<int*>(s_l + 4 * kRows) + warp * kStages;  // per stage: which groups of 16 are there
+  long long* s_pre = reinterpret_cast<long long*>(smem + ((Cfg::kFixed + 15) & ~15));  // [seqs + 1] units before
+  __shared__ long long s_scan[4];
+
+  griddep_wait();
+
+  // ---- units before each sequence
+  {
+    const int per = (bt.seqs + 127) / 128;
+    long long sum = 0;
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      if (b < bt.seqs) {
+        const Kv4Span s = kv4_span(bt, mask, b, c.page_log2);
+        sum += static_cast<long long>(s.units) * c.heads * ((s.rows * q.group + kRows - 1) / kRows);
+        s_pre[b + 1] = sum;
+      }
+    }
+    long long incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    long long before = incl - sum;
+    for (int w = 0; w < warp; ++w) before += s_scan[w];
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      if (b < bt.seqs) s_pre[b + 1] += before;
+    }
+    if (tid == 0) s_pre[0] = 0;
+    __syncthreads();
+  }
+  const long long total = s_pre[bt.seqs];
+  const long long ctas = min(static_cast<long long>(gridDim.x), total);
+  const int me = blockIdx.x;
+  if (tid == 0) desc[me] = make_int4(0, 0, 0, 0);
+  if (me >= ctas) return;
+  const long long u0 = total * me / ctas, u1 = total * (me + 1) / ctas;
+
+  auto enter = [&](Kv4Walk& w, long long unit_in_seq) {  // w.b is set
+    w.s = kv4_span(bt, mask, w.b, c.page_log2);
+    w.blocks = (w.s.rows * q.group + kRows - 1) / kRows;
+    const long long item = unit_in_seq / w.s.units;
+    w.chunk = static_cast<int>(unit_in_seq - item * w.s.units);
+    w.h = static_cast<int>(item / w.blocks);
+    w.rb = static_cast<int>(item - static_cast<long long>(w.h) * w.blocks);
+  };
+  auto advance = [&](Kv4Walk& w) {
+    if (++w.chunk < w.s.units) return;
+    w.chunk = 0;
+    if (++w.rb < w.blocks) return;
+    w.rb = 0;
+    if (++w.h < c.heads) return;
+    do ++w.b;
+    while (w.b < bt.seqs && s_pre[w.b + 1] == s_pre[w.b]);
+    if (w.b < bt.seqs) enter(w, 0);
+  };
+  Kv4Walk ld;
+  {
+    int lo = 0, hi = bt.seqs - 1;  // the sequence of unit u0: the last with s_pre <= u0 that has units
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_pre[mid] <= u0) lo = mid;
+      else hi = mid - 1;
+    }
+    ld.b = lo;
+    enter(ld, u0 - s_pre[lo]);
+  }
+  Kv4Walk cw = ld;
+
+  // ---- loads: this warp's 32 tokens of a unit into a stage of its ring
+  auto page_of = [&](const Kv4Walk& w, int group) {  // the raw page number, -1 past the end
+    const int token = w.s.base + w.chunk * kUnit + warp * 32 + group * 16;
+    return token < w.s.len ? __ldg(bt.table + static_cast<long long>(w.b) * bt.width + (token >> c.page_log2)) : -2;
+  };
+  int page0 = page_of(ld, 0), page1 = page_of(ld, 1);
+  auto issue = [&](const Kv4Walk& w, int stage) {
+    long long at[2];
+    int there = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int page = i ? page1 : page0;
+      const int token = w.s.base + w.chunk * kUnit + warp * 32 + i * 16;
+      const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
+      if (!ok && page != -2) atomicCAS(status, 0, kDevBadPage);
+      at[i] = ok ? ((static_cast<long long>(page) * c.heads + w.h) << c.page_log2) + (token & ((1 << c.page_log2) - 1)) : 0;
+      there |= ok ? 1 << i : 0;
+    }
+    if (lane == 0) s_there[stage] = there;
+    const uint32_t dst = smem_u32(ring + stage * Cfg::kStage);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int n = i * 32 + lane;
+      const int token = n / kChunks, ch = n % kChunks;
+      const int grp = token >> 4, tau = token & 15;
+      // fragment row of token tau = t + 4 a + 8 b: 2 t + a + 8 b
+      const int rho = ((tau & 3) << 1) | ((tau >> 2) & 1) | (tau & 8);
+      const int kch = D == 256 ? ch ^ ((rho & 1) << 2) : ch;
+      const int vch = D == 256 ? ch ^ ((tau & 3) << 1) : D == 128 ? ch ^ (tau & 2) : ch;
+      const long long src = ((grp ? at[1] : at[0]) + tau) * (D / 2) + ch * 16;
+      const bool ok = (there >> grp) & 1;
+      cp_async16(dst + (grp * 16 + rho) * (D / 2) + kch * 16, c.k + src, ok);
+      cp_async16(dst + Cfg::kHalf + (grp * 16 + tau) * (D / 2) + vch * 16, c.v + src, ok);
+    }
+    if (lane < 4 * kChunks) {
+      const bool is_v = lane >= 2 * kChunks;
+      const int n = is_v ? lane - 2 * kChunks : lane;
+      const int grp = n / kChunks;
+      const long long src = (grp ? at[1] : at[0]) * kChunks + (n % kChunks) * 16;
+      cp_async16(dst + 2 * Cfg::kHalf + lane * 16, (is_v ? c.vs : c.ks) + src, (there >> grp) & 1);
+    }
+  };
+  long long next = u0;  // unit of ld
+  auto issue_next = [&](int stage) {
+    if (next < u1) {
+      issue(ld, stage);
+      if (++next < u1) {
+        advance(ld);
+        page0 = page_of(ld, 0);
+        page1 = page_of(ld, 1);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) issue_next(i);
+
+  // ---- pieces
+  const float cap_k = mask.softcap > 0.f ? 2.f * kLog2e / mask.softcap : 0.f;
+  const float s_scale = mask.softcap > 0.f ? mask.scale * kTwo64 : mask.scale * kTwo64 * kLog2e;
+  int stage = 0;
+  long long u = u0;
+  while (u < u1) {
+    // Q of the item as B fragments: channels i and i + 4 of each 8 in a register, as kv4_raw gives K's
+    const int group_rows = cw.s.rows * q.group;
+    for (int i = tid; i < (D / 32) * NT * 32; i += 128) {
+      const int ln = i & 31, nt = (i >> 5) % NT, wi = (i >> 5) / NT;
+      const int r = cw.rb * kRows + nt * 8 + (ln >> 2), tt = ln & 3;
+      const int ch = D == 64 ? 16 * tt + 8 * wi : 128 * (wi >> 2) + 32 * tt + 8 * (wi & 3);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < group_rows)
+        x = __ldg(reinterpret_cast<const uint4*>(q.q + (cw.s.first + r / q.group) * q.q_row +
+                                                 (cw.h * q.group + r % q.group) * q.q_head + ch));
+      s_q[((2 * wi) * NT + nt) * 32 + ln] = make_uint2(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
+      s_q[((2 * wi + 1) * NT + nt) * 32 + ln] = make_uint2(__byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+    }
+    __syncthreads();
+    uint2 qr[NT == 1 ? D / 16 : 1];
+    if (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) qr[i] = s_q[i * 32 + lane];
+    }
+    float m[NT][2], l[NT][2], o[kMT][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
+    }
+    const int chunk0 = cw.chunk;
+    const int pb = cw.b, ph = cw.h, prb = cw.rb;
+    const Kv4Span ps = cw.s;
+    // tokens that every row of the block sees
+    const int r0 = prb * kRows, r1 = min(r0 + kRows, group_rows) - 1;
+    int all_lo, all_hi, unused;
+    kv4_visible(mask, ps.len - ps.rows + r0 / q.group, ps.len, unused, all_hi);
+    kv4_visible(mask, ps.len - ps.rows + r1 / q.group, ps.len, all_lo, unused);
+    bool more = true;
+    while (more) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      {
+        int s = stage + kStages - 1;
+        issue_next(s >= kStages ? s - kStages : s);
+      }
+      const uint8_t* kp = ring + stage * Cfg::kStage;
+      const uint8_t* vp = kp + Cfg::kHalf;
+      const uint8_t* ksp = vp + Cfg::kHalf;
+      const uint8_t* vsp = ksp + 32 * kChunks;
+      const int there = s_there[stage];
+      const int tb = ps.base + cw.chunk * kUnit + warp * 32;
+      if (there) {
+        float s[2][NT][4];
+        // ---- scores of two tiles of 16 tokens
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[tile][nt][j] = 0.f;
+          const int tau = (g >> 1) + ((g & 1) << 2);  // token of fragment row g; row g + 8: tau + 8
+          const uint8_t* row0 = kp + (tile * 16 + g) * (D / 2);
+          const uint8_t* row1 = row0 + 8 * (D / 2);
+          constexpr int kWords = D == 64 ? 2 : 4;  // codes of one scale block a thread reads at once
+#pragma unroll
+          for (int part = 0; part < (D == 256 ? 2 : 1); ++part) {
+            uint32_t w0[kWords], w1[kWords];
+            if constexpr (D == 64) {
+              const uint2 x = *reinterpret_cast<const uint2*>(row0 + t * 8), y = *reinterpret_cast<const uint2*>(row1 + t * 8);
+              w0[0] = x.x, w0[1] = x.y, w1[0] = y.x, w1[1] = y.y;
+            } else {
+              const int ch = D == 256 ? (part * 4 + t) ^ ((g & 1) << 2) : t;
+              const uint4 x = *reinterpret_cast<const uint4*>(row0 + ch * 16), y = *reinterpret_cast<const uint4*>(row1 + ch * 16);
+              w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w;
+              w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
+            }
+            const int blk = D == 64 ? t >> 1 : part * 4 + t;
+            const uint32_t f0 = kv4_scale_bf16(ksp[(tile * 16 + tau) * kChunks + blk]) * 0x10001u;
+            const uint32_t f1 = kv4_scale_bf16(ksp[(tile * 16 + tau + 8) * kChunks + blk]) * 0x10001u;
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              const uint32_t a00 = mul_bf16x2(kv4_raw<0>(w0[w]), f0), a10 = mul_bf16x2(kv4_raw<0>(w1[w]), f1);
+              const uint32_t a01 = mul_bf16x2(kv4_raw<1>(w0[w]), f0), a11 = mul_bf16x2(kv4_raw<1>(w1[w]), f1);
+              const uint32_t a02 = mul_bf16x2(kv4_raw<2>(w0[w]), f0), a12 = mul_bf16x2(kv4_raw<2>(w1[w]), f1);
+              const uint32_t a03 = mul_bf16x2(kv4_raw<3>(w0[w]), f0), a13 = mul_bf16x2(kv4_raw<3>(w1[w]), f1);
+              const int ks = 2 * (part * 4 + w);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint2 b0 = NT == 1 ? qr[ks] : s_q[(ks * NT + nt) * 32 + lane];
+                const uint2 b1 = NT == 1 ? qr[ks + 1] : s_q[((ks + 1) * NT + nt) * 32 + lane];
+                mma_bf16_16816(s[tile][nt], a00, a10, a01, a11, b0.x, b0.y);
+                mma_bf16_16816(s[tile][nt], a02, a12, a03, a13, b1.x, b1.y);
+              }
+            }
+          }
+        }
+        // ---- scale, cap, mask; running maximum
+        const bool masked = tb < all_lo || tb + 32 > all_hi || there != 3;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float top[2] = {m[nt][0], m[nt][1]};
+#pragma unroll
+          for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float x = s[tile][nt][j] * s_scale;
+              if (mask.softcap > 0.f) x = kv4_cap(x, mask.softcap, cap_k) * kLog2e;
+              s[tile][nt][j] = x;
+            }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              int lo, hi;
+              kv4_visible(mask, ps.len - ps.rows + (r0 + nt * 8 + 2 * t + e) / q.group, ps.len, lo, hi);
+#pragma unroll
+              for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const int token = tb + tile * 16 + (g >> 1) + ((g & 1) << 2) + half * 8;
+                  if (token < lo || token >= hi || !((there >> tile) & 1)) s[tile][nt][2 * half + e] = -INFINITY;
+                }
+            }
+          }
+#pragma unroll
+          for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top[j & 1] = fmaxf(top[j & 1], s[tile][nt][j]);
+#pragma unroll
+          for (int sh = 4; sh <= 16; sh <<= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], sh));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], sh));
+          }
+          if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - top[e]);
+              m[nt][e] = top[e];
+              l[nt][e] *= f;
+#pragma unroll
+              for (int i = 0; i < kMT; ++i) {
+                o[i][nt][e] *= f;
+                o[i][nt][2 + e] *= f;
+              }
+            }
+          }
+        }
+        // ---- weights to B fragments, values to A fragments
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+          uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+            const float p0 = ex2(s[tile][nt][0] - m0), p1 = ex2(s[tile][nt][1] - m1);
+            const float p2 = ex2(s[tile][nt][2] - m0), p3 = ex2(s[tile][nt][3] - m1);
+            l[nt][0] += p0 + p2;
+            l[nt][1] += p1 + p3;
+            // a weight is the sum of two bf16 numbers, to 2^-17: rounded to one alone it would add as
+            // much error to the output as the output's own rounding
+            const uint32_t h0 = pack_bf16x2(p0, p1), h1 = pack_bf16x2(p2, p3);
+            hi[nt][0] = movmatrix_trans(h0);
+            hi[nt][1] = movmatrix_trans(h1);
+            lo[nt][0] = movmatrix_trans(pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xFFFF0000u)));
+            lo[nt][1] = movmatrix_trans(pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xFFFF0000u)));
+          }
+          constexpr int kW = D / 64;  // words of codes a thread has of a token
+          uint32_t w[4][kW], f[2];    // tokens t, t + 4, t + 8, t + 12
+          uint32_t sc[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const int tau = t + 4 * a;
+            const uint8_t* row = vp + (tile * 16 + tau) * (D / 2);
+            if constexpr (D == 64) {
+              w[a][0] = *reinterpret_cast<const uint32_t*>(row + g * 4);
+            } else if constexpr (D == 128) {
+              const uint2 x = *reinterpret_cast<const uint2*>(row + (((g >> 1) ^ (tau & 2)) * 16) + (g & 1) * 8);
+              w[a][0] = x.x, w[a][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4*>(row + ((g ^ ((tau & 3) << 1)) * 16));
+              w[a][0] = x.x, w[a][1] = x.y, w[a][2] = x.z, w[a][3] = x.w;
+            }
+            sc[a] = kv4_scale_bf16(vsp[(tile * 16 + tau) * kChunks + (g * kChunks >> 3)]);
+          }
+          f[0] = sc[0] | (sc[1] << 16);
+          f[1] = sc[2] | (sc[3] << 16);
+#pragma unroll
+          for (int i = 0; i < kW; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // four channels: codes 4 half .. of word i
+              const uint32_t x0 = __byte_perm(w[0][i], w[1][i], half ? 0x7632 : 0x5410);
+              const uint32_t x1 = __byte_perm(w[2][i], w[3][i], half ? 0x7632 : 0x5410);
+              const uint32_t a0 = mul_bf16x2(kv4_raw<0>(x0), f[0]), a2 = mul_bf16x2(kv4_raw<0>(x1), f[1]);
+              const uint32_t a1 = mul_bf16x2(kv4_raw<1>(x0), f[0]), a3 = mul_bf16x2(kv4_raw<1>(x1), f[1]);
+              const uint32_t c0 = mul_bf16x2(kv4_raw<2>(x0), f[0]), c2 = mul_bf16x2(kv4_raw<2>(x1), f[1]);
+              const uint32_t c1 = mul_bf16x2(kv4_raw<3>(x0), f[0]), c3 = mul_bf16x2(kv4_raw<3>(x1), f[1]);
+              const int mt = 4 * i + 2 * half;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_bf16_16816(o[mt][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
+                mma_bf16_16816(o[mt][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+                mma_bf16_16816(o[mt + 1][nt], c0, c1, c2, c3, hi[nt][0], hi[nt][1]);
+                mma_bf16_16816(o[mt + 1][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
+              }
+            }
+        }
+      }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      ++u;
+      more = u < u1 && cw.chunk + 1 < ps.units;
+      if (more) ++cw.chunk;
+    }
+
+    // ---- the warps' parts joined
+    {
+      float* mine = s_merge + warp * kRows * Cfg::kMergeStride;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[nt][e];
+#pragma unroll
+          for (int sh = 4; sh <= 16; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+          const int r = nt * 8 + 2 * t + e;
+          if (g == 0) {
+            s_m[warp * kRows + r] = m[nt][e];
+            s_l[warp * kRows + r] = sum;
+          }
+#pragma unroll
+          for (int i = 0; i < kMT; ++i)
+            *reinterpret_cast<float2*>(mine + r * Cfg::kMergeStride + i * 16 + 2 * g) = make_float2(o[i][nt][e], o[i][nt][2 + e]);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = chunk0 == 0 && cw.chunk + 1 == ps.units;
+    float* slot = partial + (2ll * me + (u - (cw.chunk - chunk0 + 1) == u0 ? 0 : 1)) * (kRows * (D + 2));
+    for (int i = tid; i < kRows * (D / 2); i += 128) {
+      const int r = i / (D / 2), pair = i % (D / 2);
+      if (r0 + r > r1) break;
+      float top = s_m[r];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+      float sum = 0.f;
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = s_m[w * kRows + r];
+        const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
+        sum += f * s_l[w * kRows + r];
+        const float2 x = *reinterpret_cast<const float2*>(s_merge + (w * kRows + r) * Cfg::kMergeStride + 2 * pair);
+        v.x += f * x.x;
+        v.y += f * x.y;
+      }
+      // a row all of whose scores are NaN has no maximum, but a sum that is NaN
+      if (top == -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum += s_l[w * kRows + r];
+      }
+      if (whole) {
+        const long long row = ps.first + (r0 + r) / q.group;
+        const int head = ph * q.group + (r0 + r) % q.group;
+        const float f = sum == 0.f ? 0.f : kTwo64 / sum;
+        // position 16 i + 2 g + e of a warp's row is channel (D / 8) g + 2 i + e
+        const int ch = (D / 8) * (pair & 7) + 2 * (pair >> 3);
+        *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(v.x * f, v.y * f);
+        if (pair == 0) out.lse[row * q.heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) * kLn2 + logf(sum);
+      } else {
+        *reinterpret_cast<float2*>(slot + r * D + 2 * pair) = v;
+        if (pair == 0) {
+          slot[kRows * D + 2 * r] = top;
+          slot[kRows * D + 2 * r + 1] = sum;
+        }
+      }
+    }
+    if (!whole && chunk0 == 0 && tid == 0) {
+      // this CTA begins the item; the ones after it, up to the one with its last unit, go on
+      const long long last = u - 1 - cw.chunk + ps.units - 1;
+      const long long other = ((last + 1) * ctas - 1) / total;
+      desc[me] = make_int4(static_cast<int>(other) - me + 1, pb, ph * cw.blocks + prb,
+                           u - (cw.chunk - chunk0 + 1) == u0 ? 0 : 1);
+    }
+    if (u < u1) advance(cw);
+    __syncthreads();
+  }
+  griddep_launch_dependents();
+}
+
+// Joins the parts of an item that was cut: CTA i has the item that decode CTA i began.  512
+// threads: the warps share the item's rows and, where there are fewer rows than warps, its parts.
+template <int D, int NT>
+__global__ void __launch_bounds__(512)
+b2g_kv4_join_kernel(Kv4Cache c, Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial,
+                    const int4* __restrict__ desc) {
+  constexpr int kRows = 8 * NT, kE = D / 32;
+  constexpr int kShare = kRows >= 16 ? 1 : 16 / kRows;  // warps to a row
+  __shared__ float s_o[16][D];
+  __shared__ float s_m[16], s_l[16];
+  griddep_wait();
+  const int4 d = desc[blockIdx.x];
+  if (d.x == 0) return;
+  int first, end;
+  kv4_rows(bt, d.y, first, end);
+  const int group_rows = (end - first) * q.group;
+  const int blocks = (group_rows + kRows - 1) / kRows;
+  const int h = d.z / blocks, r0 = (d.z - h * blocks) * kRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = warp % kShare;
+  for (int r = warp / kShare; r < kRows; r += 16 / kShare) {
+    float top = -INFINITY, sum = 0.f, o[kE] = {};
+    if (r0 + r < group_rows) {
+      auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0 ? d.w : 0)) * (kRows * (D + 2)); };
+#pragma unroll 1
+      for (int i0 = share; i0 < d.x; i0 += 8 * kShare) {
+        float mm[8], ll[8], x[8][kE];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = i0 + j * kShare;
+          mm[j] = -INFINITY;
+          ll[j] = 0.f;
+          if (i < d.x) {
+            const float* s = slot_of(i);
+            mm[j] = s[kRows * D + 2 * r];
+            ll[j] = s[kRows * D + 2 * r + 1];
+#pragma unroll
+            for (int e = 0; e < kE; e += 2) {
+              const float2 v = *reinterpret_cast<const float2*>(s + r * D + e * 32 + 2 * lane);
+              x[j][e] = v.x;
+              x[j][e + 1] = v.y;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) x[j][e] = 0.f;
+          }
+        }
+        float t = top;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t = fmaxf(t, mm[j]);
+        const float f = top == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(top - t);
+        sum *= f;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float g = mm[j] == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(mm[j] - t);
+          sum += g * ll[j];
+#pragma unroll
+          for (int e = 0; e < kE; ++e) o[e] += g * x[j][e];
+        }
+        top = t;
+      }
+    }
+    if (kShare > 1) {
+#pragma unroll
+      for (int e = 0; e < kE; e += 2)
+        *reinterpret_cast<float2*>(&s_o[warp][e * 32 + 2 * lane]) = make_float2(o[e], o[e + 1]);
+      if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
+      __syncthreads();
+      if (share == 0) {
+        float t = top;
+        for (int w = 1; w < kShare; ++w) t = fmaxf(t, s_m[warp + w]);
+        const float f = top == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(top - t);
+        sum *= f;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] *= f;
+        for (int w = 1; w < kShare; ++w) {
+          const float mw = s_m[warp + w];
+          const float g = mw == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(mw - t);
+          sum += g * s_l[warp + w];
+#pragma unroll
+          for (int e = 0; e < kE; ++e) o[e] += g * s_o[warp + w][(e & ~1) * 32 + 2 * lane + (e & 1)];
+        }
+        top = t;
+      }
+    }
+    if (share == 0 && r0 + r < group_rows) {
+      const long long row = first + (r0 + r) / q.group;
+      const int head = h * q.group + (r0 + r) % q.group;
+      const float f = sum == 0.f ? 0.f : kTwo64 / sum;
+#pragma unroll
+      for (int e = 0; e < kE; e += 2) {
+        const int pair = e * 16 + lane;
+        const int ch = (D / 8) * (pair & 7) + 2 * (pair >> 3);
+        *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(o[e] * f, o[e + 1] * f);
+      }
+      if (lane == 0) out.lse[row * q.heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) * kLn2 + logf(sum);
+    }
+  }
+}
+
+}  // namespace b2g

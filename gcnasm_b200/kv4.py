@@ -123,23 +123,21 @@ def read(cache: KV4Cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Te
 _WORKSPACES: dict = {}
 
 
-def workspace(cache: KV4Cache, seqs: int) -> torch.Tensor:
-    """A zeroed workspace for :func:`attention` calls of up to ``seqs`` sequences: calls that may overlap
-    on the GPU need one each."""
-    n = int(capi.lib().b2g_kv4_workspace_bytes(seqs, cache.kv_heads, cache.head_dim))
+def workspace(cache: KV4Cache) -> torch.Tensor:
+    """A workspace for :func:`attention` calls, of any content: calls that may overlap on the GPU need one each."""
+    n = int(capi.lib().b2g_kv4_workspace_bytes(cache.head_dim))
     if n < 0:
         capi.check(-n, "b2g_kv4_workspace_bytes")
-    return torch.zeros(n, dtype=torch.uint8, device=cache.k.device)
+    return torch.empty(n, dtype=torch.uint8, device=cache.k.device)
 
 
-def _workspace(cache: KV4Cache, seqs: int, stream: int | None) -> torch.Tensor:
-    """The workspace this module keeps for a device and stream, grown where it is too small."""
-    key = (cache.k.device.index, stream, cache.kv_heads, cache.head_dim)
+def _workspace(cache: KV4Cache, stream: int | None) -> torch.Tensor:
+    """The workspace this module keeps for a device, stream and head_dim."""
+    key = (cache.k.device.index, stream, cache.head_dim)
     held = _WORKSPACES.get(key)
-    if held is None or held[0] < seqs:
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream or 0, device=cache.k.device)):  # zeroed in that stream's order
-            held = _WORKSPACES[key] = (seqs, workspace(cache, seqs))
-    return held[1]
+    if held is None:
+        held = _WORKSPACES[key] = workspace(cache)
+    return held
 
 
 def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch.Tensor, cu: torch.Tensor | None = None,
@@ -165,7 +163,7 @@ def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch
     lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device)
     st = _stream(stream)
     if ws is None:
-        ws = _workspace(cache, b.seqs, st.value)
+        ws = _workspace(cache, st.value)
     mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
     capi.check(capi.lib().b2g_kv4_attention(cache._args, b, mask, q.data_ptr(), q.stride(0), q.stride(1), heads,
                                             out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), ws.data_ptr(),

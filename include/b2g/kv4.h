@@ -66,7 +66,7 @@ typedef struct b2g_kv4_batch {
 
 /* Scores s = scale * q . k; softcap > 0: s = softcap * tanh(s / softcap).  The query at
  * position p (its own token's index) sees token j when j < length, j <= p (causal != 0)
- * and j > p - window (window > 0). */
+ * and j > p - window (window > 0).  scale: at most 2^60 in magnitude. */
 typedef struct b2g_kv4_mask {
     float scale;
     float softcap;
@@ -95,17 +95,16 @@ B2G_API int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch,
  * contiguous.  A query that sees no token gives out = 0, lse = -inf.  q, out: bf16,
  * element (row, head, channel) at row * *_row_stride + head * *_head_stride + channel,
  * bases and strides whole 16 bytes.  heads a multiple of kv_heads.
- * workspace: b2g_kv4_workspace_bytes(...) bytes, 16-byte aligned, zeroed once by the
- * caller before its first use; each call leaves it ready for the next.  Calls that
- * overlap on the GPU need a workspace each. */
+ * workspace: b2g_kv4_workspace_bytes(head_dim) bytes, 16-byte aligned, of any content.
+ * Calls that overlap on the GPU need a workspace each. */
 B2G_API int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask,
                               const void* q, long long q_row_stride, long long q_head_stride, int heads, void* out,
                               long long out_row_stride, long long out_head_stride, float* lse, void* workspace,
                               long long workspace_bytes, void* stream);
 
-/* Upper bound, over all lengths, of b2g_kv4_attention's workspace on the current device;
+/* Size of b2g_kv4_attention's workspace on the current device, enough for every batch;
  * negative: a status code. */
-B2G_API long long b2g_kv4_workspace_bytes(int seqs, int kv_heads, int head_dim);
+B2G_API long long b2g_kv4_workspace_bytes(int head_dim);
 
 /* Attention weight gathered by each cached token: weights_out = weights_in + sum over the
  * sequence's query rows and the kv head's query heads of exp(score - lse), for every

@@ -59,4 +59,4 @@ def test_arguments_are_refused_without_a_gpu():
     assert L.b2g_kv4_append(cache(), batch(), one, one, 0, 128, 60, 128, 64, None, None) == capi.B2G_ERR_ALIGNMENT
     assert L.b2g_kv4_append(cache(), batch(), one, one, 1, 128, 64, 126, 64, None, None) == capi.B2G_ERR_ALIGNMENT
     assert L.b2g_kv4_append(cache(), batch(lens=None), one, one, 0, 128, 64, 128, 64, None, None) == capi.B2G_ERR_INVALID_ARG
-    assert L.b2g_kv4_workspace_bytes(0, 1, 64) < 0
+    assert L.b2g_kv4_workspace_bytes(96) < 0
