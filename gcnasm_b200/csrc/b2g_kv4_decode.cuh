@@ -1,19 +1,25 @@
 // b2g_kv4_decode.cuh -- attention of few query rows over the 4-bit cache.
 //
 // For one kv head and up to 8 NT query rows (query tokens x heads of the group):
-//   S^T = K Q^T      16 tokens x 8 rows x 16 channels per mma.sync (bf16, fp32 sums)
+//   S^T = K Q^T      16 tokens x 8 rows x 16 channels per mma.sync (fp32 sums)
 //   P = 2^(S - m), m the running maximum, l the running sum (fp32)
 //   O^T += V^T P^T   16 channels x 8 rows x 16 tokens per mma.sync
 //
 // What bounds it: the cache's bytes (D + D / 16 per token and kv head).  At 6.5 TB/s an SM
-// gets ~43 codes a clock, so the codes have to become bf16 in about two integer operations
-// each; there is no time for more.  E2M1's s ee m is placed at a bf16's sign, low exponent
-// bits and top mantissa bit -- the value times 2^-126, a subnormal where e = 0 -- with shifts
-// and masks on two codes at once, and one packed multiplication by 2^(scale + 126 - 64) makes
-// it K or V times 2^-64: exact, since the scale's range is cut to 2^-60 .. 2^65.  The two
-// factors 2^64 go into the score scale and the final division.  Tensor cores here are the
-// warp-level ones: the rows of a decode step fill a sixteenth of a tcgen05 tile, and
-// its operands would have to pass through shared memory once more.
+// gets ~43 codes a clock, so there is time for two or three instructions a code.
+//   * K becomes f16: one conversion takes a byte's two codes (measured: 2.2 clocks a warp and
+//     scheduler; shifts and masks took 5.3).  The products of one 32-channel block are summed by
+//     themselves and enter the score times their scale, s += 2^sk (k . q), in fp32.  Q is brought
+//     to f16 with a power of two for each row that puts its largest element in [2^14, 2^15):
+//     exact, but for elements below 2^-29 of the row's largest, which keep an absolute
+//     precision of 2^-39 of that.
+//   * V becomes bf16, for the weights' sake: they have fp32's range, and a channel in which the
+//     heaviest tokens are zero is the sum of the light ones.  Code bits s ee m are placed at a
+//     bf16's sign, low exponent bits and top mantissa bit -- the value times 2^-126, a subnormal
+//     where e = 0 -- and a packed multiplication by 2^(sv + 126 - 64) makes it V times 2^-64:
+//     exact, since the scale's range is cut to 2^-60 .. 2^65.
+// Tensor cores here are the warp-level ones: the rows of a decode step fill a sixteenth of
+// a tcgen05 tile, and its operands would have to pass through shared memory once more.
 //
 // Tokens are dealt to warps 32 at a time: each warp keeps m, l and O for its own tokens, fed by
 // its own ring of cp.async stages, and meets the others only at the end of a piece.  Work is
@@ -79,6 +85,13 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ void mma_bf16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                                uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -92,13 +105,40 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+
+// The four bytes of w, two E2M1 codes each, as f16 pairs (low code in the low half).
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 
-// Codes I and I + 4 of a word, as bf16 values times 2^-126 (low and high half).
+// Code I of each half of w, as a bf16 value times 2^-126.
 template <int I>
 __device__ __forceinline__ uint32_t kv4_raw(uint32_t w) {
   static_assert(I >= 0 && I < 4, "four codes in each half");
@@ -107,9 +147,13 @@ __device__ __forceinline__ uint32_t kv4_raw(uint32_t w) {
   return (sign & 0x80008000u) | (mag & 0x01C001C0u);
 }
 
-// 2^(scale + 126 - 64) as a bf16, for a scale byte cut to the cache's range.
-__device__ __forceinline__ uint32_t kv4_scale_bf16(uint32_t byte) {
-  return (min(max(byte, static_cast<uint32_t>(kKv4ScaleMin)), static_cast<uint32_t>(kKv4ScaleMax)) + 62u) << 7;
+// Four scale bytes, cut to the cache's range, plus kAdd, as bf16 exponents: bytes 0 and 2, 1 and 3.
+// kAdd = 0: 2^(byte - 127); kAdd = 62: 2^(byte - 127 + 126 - 64), what turns kv4_raw's values into V 2^-64.
+template <int kAdd>
+__device__ __forceinline__ void kv4_scales_bf16(uint32_t w, uint32_t& even, uint32_t& odd) {
+  constexpr uint32_t kLo = kKv4ScaleMin * 0x10001u, kHi = kKv4ScaleMax * 0x10001u;
+  even = (__vminu2(__vmaxu2(w & 0x00FF00FFu, kLo), kHi) + kAdd * 0x10001u) << 7;
+  odd = (__vminu2(__vmaxu2((w >> 8) & 0x00FF00FFu, kLo), kHi) + kAdd * 0x10001u) << 7;
 }
 
 // ---------------------------------------------------------------------------
@@ -144,12 +188,14 @@ struct DecodeCfg {
   static constexpr int kChunks = D / 32;              // 16-byte pieces of a token's K (or V), and its scales
   static constexpr int kHalf = 32 * (D / 2);          // bytes of 32 tokens' K
   static constexpr int kStage = 2 * kHalf + 64 * kChunks;
-  // bytes in flight on an SM are CTAs x 4 warps x (stages - 1) x kStage
-  static constexpr int kStages = NT == 1 ? (D == 256 ? 3 : D == 128 ? 4 : 6) : (D == 256 ? 2 : D == 128 ? 3 : 5);
+  // Three stages of D = 128 leave room for three CTAs on an SM: 12 warps x 2 stages in flight,
+  // 104 KB where 35 KB cover the latency at full bandwidth.
+  static constexpr int kStages = D == 256 ? (NT == 1 ? 3 : 2) : D == 128 ? 3 : 5;
   static constexpr int kMergeStride = D + 4;          // fp32 row of a warp's O: rows 2t of four t in distinct banks
-  static constexpr int kMerge = 4 * kRows * kMergeStride * 4;
+  static_assert(8 * kMergeStride * 4 <= kStage, "a warp's eight rows of O lie in the stage it has just used");
   static constexpr int kQ = (D / 16) * NT * 256;      // Q as B fragments
-  static constexpr int kFixed = 4 * kStages * kStage + kMerge + kQ + 2 * 4 * kRows * 4 + 4 * kStages * 4;
+  static constexpr int kScales = 4 * 32 * kChunks;    // scales of a warp's 32 tokens as bf16
+  static constexpr int kFixed = 4 * (kStages * kStage + kScales + kStages * 4) + kQ + (2 * 4 + 2) * kRows * 4;
 };
 
 // Position of an item's units among all, walked unit by unit.
@@ -159,8 +205,18 @@ struct Kv4Walk {
   int blocks;  // row blocks of the sequence
 };
 
+// Two channels of a finished row.  Position 16 i + 2 g + e of a row of O, as the warps keep it
+// (pair = 8 i + g), is channel 32 (i / 2) + 4 g + 2 (i % 2) + e.
+__device__ __forceinline__ void kv4_finish(const Kv4Out& out, long long row, int head, int heads, int pair, float2 v, float m,
+                                           float l) {
+  const float f = l == 0.f ? 0.f : kTwo64 / l;
+  const int ch = 32 * (pair >> 4) + 4 * (pair & 7) + 2 * ((pair >> 3) & 1);
+  *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(v.x * f, v.y * f);
+  if (pair == 0) out.lse[row * heads + head] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) * kLn2 + logf(l);
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, NT == 1 && D < 256 ? 3 : 2)
 b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, float* __restrict__ partial,
                       int4* __restrict__ desc, int* status) {
   using Cfg = DecodeCfg<D, NT>;
@@ -169,11 +225,15 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * kStages * Cfg::kStage;
-  float* s_merge = reinterpret_cast<float*>(smem + 4 * kStages * Cfg::kStage);
-  uint2* s_q = reinterpret_cast<uint2*>(s_merge + Cfg::kMerge / 4);
-  float* s_m = reinterpret_cast<float*>(s_q + Cfg::kQ / 8);  // [4][kRows]
+  uint2* s_q = reinterpret_cast<uint2*>(smem + 4 * kStages * Cfg::kStage);
+  uint8_t* s_scales = reinterpret_cast<uint8_t*>(s_q) + Cfg::kQ + warp * Cfg::kScales;
+  uint8_t* s_ks = s_scales;                      // K's: [32][kChunks] bf16
+  uint16_t* s_vs = reinterpret_cast<uint16_t*>(s_scales + 64 * kChunks);  // V's: [kChunks][32] bf16
+  float* s_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + Cfg::kQ + 4 * Cfg::kScales);  // [4][kRows]
   float* s_l = s_m + 4 * kRows;
-  int* s_there = reinterpret_cast<int*>(s_l + 4 * kRows) + warp * kStages;  // per stage: which groups of 16 are there
+  float* s_rs = s_l + 4 * kRows;                 // what turns a row's sums into scores
+  int* s_top = reinterpret_cast<int*>(s_rs + kRows);
+  int* s_there = s_top + kRows + warp * kStages;  // per stage: which groups of 16 are there
   long long* s_pre = reinterpret_cast<long long*>(smem + ((Cfg::kFixed + 15) & ~15));  // [seqs + 1] units before
   __shared__ long long s_scan[4];
 
@@ -271,14 +331,13 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       const int n = i * 32 + lane;
       const int token = n / kChunks, ch = n % kChunks;
       const int grp = token >> 4, tau = token & 15;
-      // fragment row of token tau = t + 4 a + 8 b: 2 t + a + 8 b
-      const int rho = ((tau & 3) << 1) | ((tau >> 2) & 1) | (tau & 8);
-      const int kch = D == 256 ? ch ^ ((rho & 1) << 2) : ch;
-      const int vch = D == 256 ? ch ^ ((tau & 3) << 1) : D == 128 ? ch ^ (tau & 2) : ch;
+      // ldmatrix reads a piece of eight tokens at once: those eight lie in distinct banks
+      const int at_ch = ch ^ (D == 256 ? tau & 7 : D == 128 ? (tau >> 1) & 3 : (tau >> 2) & 1);
       const long long src = ((grp ? at[1] : at[0]) + tau) * (D / 2) + ch * 16;
       const bool ok = (there >> grp) & 1;
-      cp_async16(dst + (grp * 16 + rho) * (D / 2) + kch * 16, c.k + src, ok);
-      cp_async16(dst + Cfg::kHalf + (grp * 16 + tau) * (D / 2) + vch * 16, c.v + src, ok);
+      const uint32_t to = dst + token * (D / 2) + at_ch * 16;
+      cp_async16(to, c.k + src, ok);
+      cp_async16(to + Cfg::kHalf, c.v + src, ok);
     }
     if (lane < 4 * kChunks) {
       const bool is_v = lane >= 2 * kChunks;
@@ -305,34 +364,59 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 
   // ---- pieces
   const float cap_k = mask.softcap > 0.f ? 2.f * kLog2e / mask.softcap : 0.f;
-  const float s_scale = mask.softcap > 0.f ? mask.scale * kTwo64 : mask.scale * kTwo64 * kLog2e;
+  const float s_scale = mask.softcap > 0.f ? mask.scale : mask.scale * kLog2e;
+  // the token and 16-byte piece whose address this lane gives to ldmatrix
+  const int lm_tok = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
+  const uint32_t lm_row = lm_tok * (D / 2);
+  const int lm_swz = D == 256 ? lm_tok & 7 : D == 128 ? (lm_tok >> 1) & 3 : (lm_tok >> 2) & 1;
+  if (tid < kRows) s_top[tid] = 0;
+  __syncthreads();
   int stage = 0;
   long long u = u0;
   while (u < u1) {
-    // Q of the item as B fragments: channels i and i + 4 of each 8 in a register, as kv4_raw gives K's
+    // Q of the item as B fragments in f16, each row times a power of two
     const int group_rows = cw.s.rows * q.group;
+    auto q_of = [&](int i, int& r) {
+      const int ln = i & 31, nt = (i >> 5) % NT, blk = (i >> 5) / NT;
+      r = nt * 8 + (ln >> 2);
+      const int n = cw.rb * kRows + r;
+      if (n >= group_rows) return make_uint4(0, 0, 0, 0);
+      return __ldg(reinterpret_cast<const uint4*>(q.q + (cw.s.first + n / q.group) * q.q_row +
+                                                  (cw.h * q.group + n % q.group) * q.q_head + 32 * blk + 8 * (ln & 3)));
+    };
     for (int i = tid; i < (D / 32) * NT * 32; i += 128) {
-      const int ln = i & 31, nt = (i >> 5) % NT, wi = (i >> 5) / NT;
-      const int r = cw.rb * kRows + nt * 8 + (ln >> 2), tt = ln & 3;
-      const int ch = D == 64 ? 16 * tt + 8 * wi : 128 * (wi >> 2) + 32 * tt + 8 * (wi & 3);
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (r < group_rows)
-        x = __ldg(reinterpret_cast<const uint4*>(q.q + (cw.s.first + r / q.group) * q.q_row +
-                                                 (cw.h * q.group + r % q.group) * q.q_head + ch));
-      s_q[((2 * wi) * NT + nt) * 32 + ln] = make_uint2(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
-      s_q[((2 * wi + 1) * NT + nt) * 32 + ln] = make_uint2(__byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+      int r;
+      const uint4 x = q_of(i, r);
+      uint32_t top = 0;  // magnitudes as integers
+      for (uint32_t w : {x.x, x.y, x.z, x.w}) top = max(top, max((w << 16) & 0x7FFF0000u, w & 0x7FFF0000u));
+      atomicMax(&s_top[r], static_cast<int>(top));
     }
     __syncthreads();
+    for (int i = tid; i < (D / 32) * NT * 32; i += 128) {
+      int r;
+      const uint4 x = q_of(i, r);
+      const int ex = min(max(s_top[r] >> 23, 27), 254);  // the largest element is below 2^(ex - 126)
+      const float f = __int_as_float((268 - ex) << 23);  // 2^(141 - ex)
+      auto two = [&](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f); };
+      const int at = ((i >> 5) / NT * 2 * NT + (i >> 5) % NT) * 32 + (i & 31);
+      s_q[at] = make_uint2(two(x.x), two(x.y));
+      s_q[at + NT * 32] = make_uint2(two(x.z), two(x.w));
+      if ((i >> 5) / NT == 0 && (i & 3) == 0) s_rs[r] = s_scale * __int_as_float((ex - 14) << 23);
+    }
+    __syncthreads();
+    if (tid < kRows) s_top[tid] = 0;  // for the next item, behind this one's barriers
     uint2 qr[NT == 1 ? D / 16 : 1];
     if (NT == 1) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) qr[i] = s_q[i * 32 + lane];
     }
-    float m[NT][2], l[NT][2], o[kMT][NT][4];
+    float rs[NT][2], m[NT][2], l[NT][2], o[kMT][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
+      rs[nt][0] = s_rs[nt * 8 + 2 * t];
+      rs[nt][1] = s_rs[nt * 8 + 2 * t + 1];
 #pragma unroll
       for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -355,52 +439,67 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         issue_next(s >= kStages ? s - kStages : s);
       }
       const uint8_t* kp = ring + stage * Cfg::kStage;
-      const uint8_t* vp = kp + Cfg::kHalf;
-      const uint8_t* ksp = vp + Cfg::kHalf;
-      const uint8_t* vsp = ksp + 32 * kChunks;
       const int there = s_there[stage];
       const int tb = ps.base + cw.chunk * kUnit + warp * 32;
       if (there) {
+        // ---- scales: lane i has token i's
+        {
+          const uint8_t* raw = kp + 2 * Cfg::kHalf + lane * kChunks;
+          uint32_t even, odd;
+          if constexpr (D == 64) {
+            kv4_scales_bf16<0>(*reinterpret_cast<const uint16_t*>(raw), even, odd);
+            *reinterpret_cast<uint32_t*>(s_ks + lane * 4) = __byte_perm(even, odd, 0x5410);
+            kv4_scales_bf16<62>(*reinterpret_cast<const uint16_t*>(raw + 32 * kChunks), even, odd);
+            s_vs[lane] = static_cast<uint16_t>(even);
+            s_vs[32 + lane] = static_cast<uint16_t>(odd);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kChunks / 4; ++i) {
+              kv4_scales_bf16<0>(*reinterpret_cast<const uint32_t*>(raw + 4 * i), even, odd);
+              *reinterpret_cast<uint2*>(s_ks + lane * kChunks * 2 + i * 8) = make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+              kv4_scales_bf16<62>(*reinterpret_cast<const uint32_t*>(raw + 32 * kChunks + 4 * i), even, odd);
+              s_vs[(4 * i) * 32 + lane] = static_cast<uint16_t>(even);
+              s_vs[(4 * i + 1) * 32 + lane] = static_cast<uint16_t>(odd);
+              s_vs[(4 * i + 2) * 32 + lane] = static_cast<uint16_t>(even >> 16);
+              s_vs[(4 * i + 3) * 32 + lane] = static_cast<uint16_t>(odd >> 16);
+            }
+          }
+          __syncwarp();
+        }
         float s[2][NT][4];
+        const uint32_t k_at = smem_u32(kp) + lm_row;
         // ---- scores of two tiles of 16 tokens
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
+          const uint8_t* sr0 = s_ks + (tile * 16 + g) * kChunks * 2;
+          const uint8_t* sr1 = sr0 + 8 * kChunks * 2;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int pair = 0; pair < kChunks / 2; ++pair) {  // two blocks of channels
+            uint32_t kw[4];  // tokens g and g + 8 of the first block, then of the second
+            ldmatrix_x4(kw, k_at + tile * 16 * (D / 2) + (((2 * pair + lm_ch) ^ lm_swz) * 16));
+            const uint32_t f0 = *reinterpret_cast<const uint32_t*>(sr0 + pair * 4), f1 = *reinterpret_cast<const uint32_t*>(sr1 + pair * 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[tile][nt][j] = 0.f;
-          const int tau = (g >> 1) + ((g & 1) << 2);  // token of fragment row g; row g + 8: tau + 8
-          const uint8_t* row0 = kp + (tile * 16 + g) * (D / 2);
-          const uint8_t* row1 = row0 + 8 * (D / 2);
-          constexpr int kWords = D == 64 ? 2 : 4;  // codes of one scale block a thread reads at once
-#pragma unroll
-          for (int part = 0; part < (D == 256 ? 2 : 1); ++part) {
-            uint32_t w0[kWords], w1[kWords];
-            if constexpr (D == 64) {
-              const uint2 x = *reinterpret_cast<const uint2*>(row0 + t * 8), y = *reinterpret_cast<const uint2*>(row1 + t * 8);
-              w0[0] = x.x, w0[1] = x.y, w1[0] = y.x, w1[1] = y.y;
-            } else {
-              const int ch = D == 256 ? (part * 4 + t) ^ ((g & 1) << 2) : t;
-              const uint4 x = *reinterpret_cast<const uint4*>(row0 + ch * 16), y = *reinterpret_cast<const uint4*>(row1 + ch * 16);
-              w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w;
-              w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
-            }
-            const int blk = D == 64 ? t >> 1 : part * 4 + t;
-            const uint32_t f0 = kv4_scale_bf16(ksp[(tile * 16 + tau) * kChunks + blk]) * 0x10001u;
-            const uint32_t f1 = kv4_scale_bf16(ksp[(tile * 16 + tau + 8) * kChunks + blk]) * 0x10001u;
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              const uint32_t a00 = mul_bf16x2(kv4_raw<0>(w0[w]), f0), a10 = mul_bf16x2(kv4_raw<0>(w1[w]), f1);
-              const uint32_t a01 = mul_bf16x2(kv4_raw<1>(w0[w]), f0), a11 = mul_bf16x2(kv4_raw<1>(w1[w]), f1);
-              const uint32_t a02 = mul_bf16x2(kv4_raw<2>(w0[w]), f0), a12 = mul_bf16x2(kv4_raw<2>(w1[w]), f1);
-              const uint32_t a03 = mul_bf16x2(kv4_raw<3>(w0[w]), f0), a13 = mul_bf16x2(kv4_raw<3>(w1[w]), f1);
-              const int ks = 2 * (part * 4 + w);
+            for (int half = 0; half < 2; ++half) {
+              const int blk = 2 * pair + half;
+              uint32_t a[4], b[4];
+              e2m1x8_to_f16(kw[2 * half], a);
+              e2m1x8_to_f16(kw[2 * half + 1], b);
+              const float g0 = __uint_as_float(half ? f0 & 0xFFFF0000u : f0 << 16);
+              const float g1 = __uint_as_float(half ? f1 & 0xFFFF0000u : f1 << 16);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                const uint2 b0 = NT == 1 ? qr[ks] : s_q[(ks * NT + nt) * 32 + lane];
-                const uint2 b1 = NT == 1 ? qr[ks + 1] : s_q[((ks + 1) * NT + nt) * 32 + lane];
-                mma_bf16_16816(s[tile][nt], a00, a10, a01, a11, b0.x, b0.y);
-                mma_bf16_16816(s[tile][nt], a02, a12, a03, a13, b1.x, b1.y);
+                const uint2 b0 = NT == 1 ? qr[2 * blk] : s_q[(2 * blk * NT + nt) * 32 + lane];
+                const uint2 b1 = NT == 1 ? qr[2 * blk + 1] : s_q[((2 * blk + 1) * NT + nt) * 32 + lane];
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16_16816(x, a[0], b[0], a[1], b[1], b0.x, b0.y);
+                mma_f16_16816(x, a[2], b[2], a[3], b[3], b1.x, b1.y);
+                if (blk == 0) {
+                  s[tile][nt][0] = x[0] * g0, s[tile][nt][1] = x[1] * g0;
+                  s[tile][nt][2] = x[2] * g1, s[tile][nt][3] = x[3] * g1;
+                } else {
+                  s[tile][nt][0] = fmaf(x[0], g0, s[tile][nt][0]), s[tile][nt][1] = fmaf(x[1], g0, s[tile][nt][1]);
+                  s[tile][nt][2] = fmaf(x[2], g1, s[tile][nt][2]), s[tile][nt][3] = fmaf(x[3], g1, s[tile][nt][3]);
+                }
               }
             }
           }
@@ -414,7 +513,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
           for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float x = s[tile][nt][j] * s_scale;
+              float x = s[tile][nt][j] * rs[nt][j & 1];
               if (mask.softcap > 0.f) x = kv4_cap(x, mask.softcap, cap_k) * kLog2e;
               s[tile][nt][j] = x;
             }
@@ -427,7 +526,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
               for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                  const int token = tb + tile * 16 + (g >> 1) + ((g & 1) << 2) + half * 8;
+                  const int token = tb + tile * 16 + g + half * 8;
                   if (token < lo || token >= hi || !((there >> tile) & 1)) s[tile][nt][2 * half + e] = -INFINITY;
                 }
             }
@@ -455,7 +554,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
             }
           }
         }
-        // ---- weights to B fragments, values to A fragments
+        // ---- weights, and their product with V
+        const uint32_t v_at = k_at + Cfg::kHalf;
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile) {
           uint32_t hi[NT][2], lo[NT][2];
@@ -474,45 +574,30 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
             lo[nt][0] = movmatrix_trans(pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xFFFF0000u)));
             lo[nt][1] = movmatrix_trans(pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xFFFF0000u)));
           }
-          constexpr int kW = D / 64;  // words of codes a thread has of a token
-          uint32_t w[4][kW], f[2];    // tokens t, t + 4, t + 8, t + 12
-          uint32_t sc[4];
 #pragma unroll
-          for (int a = 0; a < 4; ++a) {
-            const int tau = t + 4 * a;
-            const uint8_t* row = vp + (tile * 16 + tau) * (D / 2);
-            if constexpr (D == 64) {
-              w[a][0] = *reinterpret_cast<const uint32_t*>(row + g * 4);
-            } else if constexpr (D == 128) {
-              const uint2 x = *reinterpret_cast<const uint2*>(row + (((g >> 1) ^ (tau & 2)) * 16) + (g & 1) * 8);
-              w[a][0] = x.x, w[a][1] = x.y;
-            } else {
-              const uint4 x = *reinterpret_cast<const uint4*>(row + ((g ^ ((tau & 3) << 1)) * 16));
-              w[a][0] = x.x, w[a][1] = x.y, w[a][2] = x.z, w[a][3] = x.w;
-            }
-            sc[a] = kv4_scale_bf16(vsp[(tile * 16 + tau) * kChunks + (g * kChunks >> 3)]);
-          }
-          f[0] = sc[0] | (sc[1] << 16);
-          f[1] = sc[2] | (sc[3] << 16);
+          for (int pair = 0; pair < kChunks / 2; ++pair) {
+            // codes 4 g .. 4 g + 3 of a block: tokens 2 t | 2 t + 1, then 2 t + 8 | 2 t + 9
+            uint32_t vw[4];
+            ldmatrix_x4_trans(vw, v_at + tile * 16 * (D / 2) + (((2 * pair + lm_ch) ^ lm_swz) * 16));
 #pragma unroll
-          for (int i = 0; i < kW; ++i)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // four channels: codes 4 half .. of word i
-              const uint32_t x0 = __byte_perm(w[0][i], w[1][i], half ? 0x7632 : 0x5410);
-              const uint32_t x1 = __byte_perm(w[2][i], w[3][i], half ? 0x7632 : 0x5410);
-              const uint32_t a0 = mul_bf16x2(kv4_raw<0>(x0), f[0]), a2 = mul_bf16x2(kv4_raw<0>(x1), f[1]);
-              const uint32_t a1 = mul_bf16x2(kv4_raw<1>(x0), f[0]), a3 = mul_bf16x2(kv4_raw<1>(x1), f[1]);
-              const uint32_t c0 = mul_bf16x2(kv4_raw<2>(x0), f[0]), c2 = mul_bf16x2(kv4_raw<2>(x1), f[1]);
-              const uint32_t c1 = mul_bf16x2(kv4_raw<3>(x0), f[0]), c3 = mul_bf16x2(kv4_raw<3>(x1), f[1]);
-              const int mt = 4 * i + 2 * half;
+            for (int half = 0; half < 2; ++half) {
+              const int blk = 2 * pair + half;
+              const uint32_t f0 = *reinterpret_cast<const uint32_t*>(s_vs + blk * 32 + tile * 16 + 2 * t);
+              const uint32_t f1 = *reinterpret_cast<const uint32_t*>(s_vs + blk * 32 + tile * 16 + 2 * t + 8);
+              const uint32_t x0 = vw[2 * half], x1 = vw[2 * half + 1];
+              const uint32_t a0 = mul_bf16x2(kv4_raw<0>(x0), f0), a2 = mul_bf16x2(kv4_raw<0>(x1), f1);
+              const uint32_t a1 = mul_bf16x2(kv4_raw<1>(x0), f0), a3 = mul_bf16x2(kv4_raw<1>(x1), f1);
+              const uint32_t c0 = mul_bf16x2(kv4_raw<2>(x0), f0), c2 = mul_bf16x2(kv4_raw<2>(x1), f1);
+              const uint32_t c1 = mul_bf16x2(kv4_raw<3>(x0), f0), c3 = mul_bf16x2(kv4_raw<3>(x1), f1);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma_bf16_16816(o[mt][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
-                mma_bf16_16816(o[mt][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
-                mma_bf16_16816(o[mt + 1][nt], c0, c1, c2, c3, hi[nt][0], hi[nt][1]);
-                mma_bf16_16816(o[mt + 1][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
+                mma_bf16_16816(o[2 * blk][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
+                mma_bf16_16816(o[2 * blk][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+                mma_bf16_16816(o[2 * blk + 1][nt], c0, c1, c2, c3, hi[nt][0], hi[nt][1]);
+                mma_bf16_16816(o[2 * blk + 1][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
               }
             }
+          }
         }
       }
       stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -521,67 +606,60 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       if (more) ++cw.chunk;
     }
 
-    // ---- the warps' parts joined
-    {
-      float* mine = s_merge + warp * kRows * Cfg::kMergeStride;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float sum = l[nt][e];
-#pragma unroll
-          for (int sh = 4; sh <= 16; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
-          const int r = nt * 8 + 2 * t + e;
-          if (g == 0) {
-            s_m[warp * kRows + r] = m[nt][e];
-            s_l[warp * kRows + r] = sum;
-          }
-#pragma unroll
-          for (int i = 0; i < kMT; ++i)
-            *reinterpret_cast<float2*>(mine + r * Cfg::kMergeStride + i * 16 + 2 * g) = make_float2(o[i][nt][e], o[i][nt][2 + e]);
-        }
-      }
-    }
-    __syncthreads();
+    // ---- the warps' parts joined, eight rows at a time, through the stages just used
     const bool whole = chunk0 == 0 && cw.chunk + 1 == ps.units;
     float* slot = partial + (2ll * me + (u - (cw.chunk - chunk0 + 1) == u0 ? 0 : 1)) * (kRows * (D + 2));
-    for (int i = tid; i < kRows * (D / 2); i += 128) {
-      const int r = i / (D / 2), pair = i % (D / 2);
-      if (r0 + r > r1) break;
-      float top = s_m[r];
+    const int used = (stage == 0 ? kStages : stage) - 1;
+    __syncwarp();
 #pragma unroll
-      for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * kRows + r]);
-      float sum = 0.f;
-      float2 v = make_float2(0.f, 0.f);
+    for (int nt = 0; nt < NT; ++nt) {
+      float* mine = reinterpret_cast<float*>(ring + used * Cfg::kStage);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = s_m[w * kRows + r];
-        const float f = mw == -INFINITY ? 0.f : ex2(mw - top);
-        sum += f * s_l[w * kRows + r];
-        const float2 x = *reinterpret_cast<const float2*>(s_merge + (w * kRows + r) * Cfg::kMergeStride + 2 * pair);
-        v.x += f * x.x;
-        v.y += f * x.y;
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int sh = 4; sh <= 16; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+        if (g == 0) {
+          s_m[warp * kRows + nt * 8 + 2 * t + e] = m[nt][e];
+          s_l[warp * kRows + nt * 8 + 2 * t + e] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < kMT; ++i)
+          *reinterpret_cast<float2*>(mine + (2 * t + e) * Cfg::kMergeStride + i * 16 + 2 * g) = make_float2(o[i][nt][e], o[i][nt][2 + e]);
       }
-      // a row all of whose scores are NaN has no maximum, but a sum that is NaN
-      if (top == -INFINITY) {
+      __syncthreads();
+      for (int i = tid; i < 8 * (D / 2); i += 128) {
+        const int r = nt * 8 + i / (D / 2), pair = i % (D / 2);
+        if (r0 + r > r1) break;
+        float top = s_m[r];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) sum += s_l[w * kRows + r];
-      }
-      if (whole) {
-        const long long row = ps.first + (r0 + r) / q.group;
-        const int head = ph * q.group + (r0 + r) % q.group;
-        const float f = sum == 0.f ? 0.f : kTwo64 / sum;
-        // position 16 i + 2 g + e of a warp's row is channel (D / 8) g + 2 i + e
-        const int ch = (D / 8) * (pair & 7) + 2 * (pair >> 3);
-        *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(v.x * f, v.y * f);
-        if (pair == 0) out.lse[row * q.heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) * kLn2 + logf(sum);
-      } else {
-        *reinterpret_cast<float2*>(slot + r * D + 2 * pair) = v;
-        if (pair == 0) {
-          slot[kRows * D + 2 * r] = top;
-          slot[kRows * D + 2 * r + 1] = sum;
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+        float sum = 0.f;
+        float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float mw = s_m[w * kRows + r];
+          // a row all of whose scores are NaN has no maximum, but a sum that is NaN
+          const float f = mw == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : ex2(mw - top);
+          sum += f * s_l[w * kRows + r];
+          const float2 x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem + (w * kStages + used) * Cfg::kStage) +
+                                                            (r - nt * 8) * Cfg::kMergeStride + 2 * pair);
+          v.x += f * x.x;
+          v.y += f * x.y;
+        }
+        if (whole) {
+          const long long row = ps.first + (r0 + r) / q.group;
+          const int head = ph * q.group + (r0 + r) % q.group;
+          kv4_finish(out, row, head, q.heads, pair, v, top, sum);
+        } else {
+          *reinterpret_cast<float2*>(slot + r * D + 2 * pair) = v;
+          if (pair == 0) {
+            slot[kRows * D + 2 * r] = top;
+            slot[kRows * D + 2 * r + 1] = sum;
+          }
         }
       }
+      __syncthreads();
     }
     if (!whole && chunk0 == 0 && tid == 0) {
       // this CTA begins the item; the ones after it, up to the one with its last unit, go on
@@ -591,7 +669,6 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
                            u - (cw.chunk - chunk0 + 1) == u0 ? 0 : 1);
     }
     if (u < u1) advance(cw);
-    __syncthreads();
   }
   griddep_launch_dependents();
 }
@@ -686,14 +763,8 @@ b2g_kv4_join_kernel(Kv4Cache c, Kv4Batch bt, Kv4Queries q, Kv4Out out, const flo
     if (share == 0 && r0 + r < group_rows) {
       const long long row = first + (r0 + r) / q.group;
       const int head = h * q.group + (r0 + r) % q.group;
-      const float f = sum == 0.f ? 0.f : kTwo64 / sum;
 #pragma unroll
-      for (int e = 0; e < kE; e += 2) {
-        const int pair = e * 16 + lane;
-        const int ch = (D / 8) * (pair & 7) + 2 * (pair >> 3);
-        *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(o[e] * f, o[e + 1] * f);
-      }
-      if (lane == 0) out.lse[row * q.heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) * kLn2 + logf(sum);
+      for (int e = 0; e < kE; e += 2) kv4_finish(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), top, sum);
     }
   }
 }
