@@ -158,6 +158,16 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   return launch(b2g_kv4_join_kernel<D, NT>, dim3(grid), 512, 0, f.st, f.c, f.bt, q, o, partial, desc);
 }
 
+template <int D>
+int gather(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const float* lse, const float* w_in, float* w_out) {
+  static std::atomic<int> few[64], many[64];
+  const bool is_few = f.bt.seqs <= 512;
+  const size_t smem = ((WeightsCfg<D>::kFixed + 15) & ~15) + ((is_few ? 512 : 8192) + 1) * sizeof(long long);
+  const int n = resident(b2g_kv4_weights_kernel<D>, 128, smem, 16, f.dev, is_few ? few : many);
+  if (n < 1) return host_fail(B2G_ERR_CUDA, "the weights kernel does not fit on the device");
+  return launch(b2g_kv4_weights_kernel<D>, dim3(n * f.sms), 128, smem, f.st, f.c, f.bt, m, q, lse, w_in, w_out, f.status);
+}
+
 }  // namespace
 
 extern "C" {
@@ -254,10 +264,9 @@ int b2g_kv4_weights(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, cons
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    b2g_kv4_weights_kernel<D><<<dim3(64, f.c.heads, f.bt.seqs), 128, 0, f.st>>>(f.c, f.bt, m, qs, lse, weights_in, weights_out,
-                                                                               f.status);
+    rc = gather<D>(f, m, qs, lse, weights_in, weights_out);
   });
-  return launched();
+  return rc;
 }
 
 int b2g_kv4_evict(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, float* weights, int budget, int sink, int recent,

@@ -182,6 +182,85 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& bt, const Kv4Mask& m
   return s;
 }
 
+// Units before each sequence, pre[0 .. seqs], by a CTA of 128 threads: each takes some
+// consecutive sequences.
+template <typename F>
+__device__ __forceinline__ void kv4_scan(int seqs, long long* pre, long long* warp_sum, F&& units) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (seqs + 127) / 128;
+  long long sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < seqs) {
+      sum += units(b);
+      pre[b + 1] = sum;
+    }
+  }
+  long long incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  long long before = incl - sum;
+  for (int w = 0; w < warp; ++w) before += warp_sum[w];
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < seqs) pre[b + 1] += before;
+  }
+  if (tid == 0) pre[0] = 0;
+  __syncthreads();
+}
+
+// The last sequence whose units begin at or before `unit` (the one that has it: empty ones do not come last).
+__device__ __forceinline__ int kv4_seq_of_unit(const long long* pre, int seqs, long long unit) {
+  int lo = 0, hi = seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= unit) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// 8 NT query rows of a kv head, from row n0 of its group_rows, as B fragments in f16: each row
+// times a power of two that puts its largest element in [2^14, 2^15), whose inverse times `scale`
+// goes to s_rs.  s_top: zeros, 8 NT, and the caller clears it behind the barrier that follows.
+template <int D, int NT, int kThreads>
+__device__ __forceinline__ void kv4_stage_q(const Kv4Queries& q, int first, int h, int n0, int group_rows, float scale, uint2* s_q,
+                                            int* s_top, float* s_rs) {
+  auto q_of = [&](int i, int& r) {
+    const int ln = i & 31, nt = (i >> 5) % NT, blk = (i >> 5) / NT;
+    r = nt * 8 + (ln >> 2);
+    const int n = n0 + r;
+    if (n >= group_rows) return make_uint4(0, 0, 0, 0);
+    return __ldg(reinterpret_cast<const uint4*>(q.q + (first + n / q.group) * q.q_row + (h * q.group + n % q.group) * q.q_head +
+                                                32 * blk + 8 * (ln & 3)));
+  };
+  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += kThreads) {
+    int r;
+    const uint4 x = q_of(i, r);
+    uint32_t top = 0;  // magnitudes as integers
+    for (uint32_t w : {x.x, x.y, x.z, x.w}) top = max(top, max((w << 16) & 0x7FFF0000u, w & 0x7FFF0000u));
+    atomicMax(&s_top[r], static_cast<int>(top));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += kThreads) {
+    int r;
+    const uint4 x = q_of(i, r);
+    const int ex = min(max(s_top[r] >> 23, 27), 254);  // the largest element is below 2^(ex - 126)
+    const float f = __int_as_float((268 - ex) << 23);  // 2^(141 - ex)
+    auto two = [&](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f); };
+    const int at = ((i >> 5) / NT * 2 * NT + (i >> 5) % NT) * 32 + (i & 31);
+    s_q[at] = make_uint2(two(x.x), two(x.y));
+    s_q[at + NT * 32] = make_uint2(two(x.z), two(x.w));
+    if ((i >> 5) / NT == 0 && (i & 3) == 0) s_rs[r] = scale * __int_as_float((ex - 14) << 23);
+  }
+  __syncthreads();
+}
+
 template <int D, int NT>
 struct DecodeCfg {
   static constexpr int kRows = 8 * NT;
@@ -239,35 +318,10 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 
   griddep_wait();
 
-  // ---- units before each sequence
-  {
-    const int per = (bt.seqs + 127) / 128;
-    long long sum = 0;
-    for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i;
-      if (b < bt.seqs) {
-        const Kv4Span s = kv4_span(bt, mask, b, c.page_log2);
-        sum += static_cast<long long>(s.units) * c.heads * ((s.rows * q.group + kRows - 1) / kRows);
-        s_pre[b + 1] = sum;
-      }
-    }
-    long long incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    long long before = incl - sum;
-    for (int w = 0; w < warp; ++w) before += s_scan[w];
-    for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i;
-      if (b < bt.seqs) s_pre[b + 1] += before;
-    }
-    if (tid == 0) s_pre[0] = 0;
-    __syncthreads();
-  }
+  kv4_scan(bt.seqs, s_pre, s_scan, [&](int b) {
+    const Kv4Span s = kv4_span(bt, mask, b, c.page_log2);
+    return static_cast<long long>(s.units) * c.heads * ((s.rows * q.group + kRows - 1) / kRows);
+  });
   const long long total = s_pre[bt.seqs];
   const long long ctas = min(static_cast<long long>(gridDim.x), total);
   const int me = blockIdx.x;
@@ -295,12 +349,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   };
   Kv4Walk ld;
   {
-    int lo = 0, hi = bt.seqs - 1;  // the sequence of unit u0: the last with s_pre <= u0 that has units
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_pre[mid] <= u0) lo = mid;
-      else hi = mid - 1;
-    }
+    const int lo = kv4_seq_of_unit(s_pre, bt.seqs, u0);
     ld.b = lo;
     enter(ld, u0 - s_pre[lo]);
   }
@@ -374,36 +423,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   int stage = 0;
   long long u = u0;
   while (u < u1) {
-    // Q of the item as B fragments in f16, each row times a power of two
     const int group_rows = cw.s.rows * q.group;
-    auto q_of = [&](int i, int& r) {
-      const int ln = i & 31, nt = (i >> 5) % NT, blk = (i >> 5) / NT;
-      r = nt * 8 + (ln >> 2);
-      const int n = cw.rb * kRows + r;
-      if (n >= group_rows) return make_uint4(0, 0, 0, 0);
-      return __ldg(reinterpret_cast<const uint4*>(q.q + (cw.s.first + n / q.group) * q.q_row +
-                                                  (cw.h * q.group + n % q.group) * q.q_head + 32 * blk + 8 * (ln & 3)));
-    };
-    for (int i = tid; i < (D / 32) * NT * 32; i += 128) {
-      int r;
-      const uint4 x = q_of(i, r);
-      uint32_t top = 0;  // magnitudes as integers
-      for (uint32_t w : {x.x, x.y, x.z, x.w}) top = max(top, max((w << 16) & 0x7FFF0000u, w & 0x7FFF0000u));
-      atomicMax(&s_top[r], static_cast<int>(top));
-    }
-    __syncthreads();
-    for (int i = tid; i < (D / 32) * NT * 32; i += 128) {
-      int r;
-      const uint4 x = q_of(i, r);
-      const int ex = min(max(s_top[r] >> 23, 27), 254);  // the largest element is below 2^(ex - 126)
-      const float f = __int_as_float((268 - ex) << 23);  // 2^(141 - ex)
-      auto two = [&](uint32_t w) { return pack_f16x2(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xFFFF0000u) * f); };
-      const int at = ((i >> 5) / NT * 2 * NT + (i >> 5) % NT) * 32 + (i & 31);
-      s_q[at] = make_uint2(two(x.x), two(x.y));
-      s_q[at + NT * 32] = make_uint2(two(x.z), two(x.w));
-      if ((i >> 5) / NT == 0 && (i & 3) == 0) s_rs[r] = s_scale * __int_as_float((ex - 14) << 23);
-    }
-    __syncthreads();
+    kv4_stage_q<D, NT, 128>(q, cw.s.first, cw.h, cw.rb * kRows, group_rows, s_scale, s_q, s_top, s_rs);
     if (tid < kRows) s_top[tid] = 0;  // for the next item, behind this one's barriers
     uint2 qr[NT == 1 ? D / 16 : 1];
     if (NT == 1) {
