@@ -1170,6 +1170,8 @@ int host_device(int* sms, int** status, int* dev) {
   return B2G_OK;
 }
 
+unsigned long long host_wait_timeout_ns() { return g_timeout_ns.load(); }
+
 }  // namespace b2g
 
 extern "C" {

@@ -10,4 +10,7 @@ int host_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3
 // SM count, status word and number (0 .. 63) of the current device (an sm_100 one); a status code
 int host_device(int* sms, int** status, int* dev = nullptr);
 
+// how long a kernel's bounded wait lasts (b2g_set_wait_timeout_ms)
+unsigned long long host_wait_timeout_ns();
+
 }  // namespace b2g

@@ -11,6 +11,7 @@
 #include "b2g_host.h"
 #include "b2g_kv4.cuh"
 #include "b2g_kv4_decode.cuh"
+#include "b2g_kv4_prompt.cuh"
 #include "b2g_kv4_weights.cuh"
 
 using namespace b2g;
@@ -125,6 +126,9 @@ long long decode_workspace(int sms, int dim) {
   return most;
 }
 
+// From this many rows of a kv head on, the tcgen05 kernel
+constexpr long long kPromptRows = 64;
+
 // Resident CTAs per SM, at most `most`, of a kernel with `smem` dynamic bytes on the current
 // device; 0: it does not fit.  Asked of the runtime once per kernel, device and size class.
 template <typename K>
@@ -156,6 +160,18 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   int rc = launch(b2g_kv4_decode_kernel<D, NT>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
   if (rc) return rc;
   return launch(b2g_kv4_join_kernel<D, NT>, dim3(grid), 512, 0, f.st, f.c, f.bt, q, o, partial, desc);
+}
+
+template <int D>
+int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, long long group_rows) {
+  using Cfg = PromptCfg<D>;
+  static std::atomic<int> known[64];
+  if (resident(b2g_kv4_prompt_kernel<D>, Cfg::kThreads, Cfg::kSmem, 1, f.dev, known) < 1)
+    return host_fail(B2G_ERR_CUDA, "the prompt kernel does not fit on the device");
+  const long long blocks = (group_rows + Cfg::kRows - 1) / Cfg::kRows;
+  if (blocks > 65535) return host_fail(B2G_ERR_UNSUPPORTED, "max_new %lld x the heads of a group is beyond %d rows", group_rows, 65535 * Cfg::kRows);
+  return launch(b2g_kv4_prompt_kernel<D>, dim3(f.c.heads, f.bt.seqs, static_cast<unsigned>(blocks)), Cfg::kThreads, Cfg::kSmem, f.st,
+                f.c, f.bt, m, q, o, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
 }
 
 template <int D>
@@ -241,10 +257,11 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
   const Kv4Out o{static_cast<__nv_bfloat16*>(out), out_row_stride, out_head_stride, lse};
-  const long long rows = static_cast<long long>(std::max(1, batch->cu ? batch->max_new : 1)) * qs.group;
+  const long long rows = static_cast<long long>(std::max(1, batch->cu ? std::min(batch->max_new, batch->rows) : 1)) * qs.group;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (rows <= 8) rc = decode<D, 1>(f, m, qs, o, workspace);
+    if (rows >= kPromptRows) rc = prompt<D>(f, m, qs, o, rows);
+    else if (rows <= 8) rc = decode<D, 1>(f, m, qs, o, workspace);
     else if (rows <= 16 || D == 256) rc = decode<D, 2>(f, m, qs, o, workspace);
     else if constexpr (D < 256) rc = decode<D, 4>(f, m, qs, o, workspace);
   });
