@@ -16,7 +16,6 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from .ops import _stream
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -56,31 +55,55 @@ def alloc_weights(cache: KV4Cache) -> torch.Tensor:
     return torch.zeros((cache.pages, cache.kv_heads, cache.page_size), dtype=torch.float32, device=cache.k.device)
 
 
-def _ints(t: torch.Tensor, name: str, dim: int, size: int | None = None) -> int:
-    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous() or t.dim() != dim:
-        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of {dim} dimension(s)")
-    if size is not None and t.shape[0] != size:
+# A decode step makes several of these calls on a few microseconds' work each, so the checks
+# below read every attribute once and build nothing they do not pass on.
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+
+def _raw_stream(stream, device: torch.device) -> int:
+    """The cudaStream_t of `stream`, or of the device's current one."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _ints(t: torch.Tensor, name: str, size: int) -> int:
+    if t.dtype is not _I32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of one dimension")
+    if t.shape[0] != size:
         raise ValueError(f"{name} has {t.shape[0]} entries, not {size}")
     return t.data_ptr()
 
 
+def _table(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(address, sequences, pages a sequence)"""
+    if t.dtype is not _I32 or not t.is_cuda or t.dim() != 2 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor [sequences, pages]")
+    seqs, width = t.shape
+    return t.data_ptr(), seqs, width
+
+
 def _batch(table, lens, cu, rows: int, max_new: int | None) -> capi.Kv4Batch:
-    tp = _ints(table, "table", 2)
-    seqs, width = table.shape
-    lp = _ints(lens, "lens", 1, seqs) if lens is not None else None
-    cp = _ints(cu, "cu", 1, seqs + 1) if cu is not None else None
+    tp, seqs, width = _table(table, "table")
+    lp = _ints(lens, "lens", seqs) if lens is not None else None
+    cp = _ints(cu, "cu", seqs + 1) if cu is not None else None
     if max_new is None:
         max_new = rows if cu is not None else 1
     return capi.Kv4Batch(tp, lp, cp, seqs, width, rows, max_new)
 
 
-def _heads(t: torch.Tensor, name: str, cache: KV4Cache) -> None:
-    if t.dim() != 3 or not t.is_cuda or t.shape[2] != cache.head_dim or t.stride(2) != 1:
-        raise ValueError(f"{name} must be a CUDA tensor [rows, heads, {cache.head_dim}] with unit channel stride")
+def _heads(t: torch.Tensor, name: str, cache: KV4Cache) -> tuple[int, int, int, int]:
+    """(rows, heads, row stride, head stride)"""
+    if t.dim() == 3 and t.is_cuda:
+        rows, heads, dim = t.shape
+        row, head, one = t.stride()
+        if dim == cache.head_dim and one == 1:
+            return rows, heads, row, head
+    raise ValueError(f"{name} must be a CUDA tensor [rows, heads, {cache.head_dim}] with unit channel stride")
 
 
 def _weights_array(t: torch.Tensor, name: str, cache: KV4Cache) -> int:
-    if t.dtype is not torch.float32 or not t.is_cuda or not t.is_contiguous() or \
+    if t.dtype is not _F32 or not t.is_cuda or not t.is_contiguous() or \
             t.shape != (cache.pages, cache.kv_heads, cache.page_size):
         raise ValueError(f"{name} must be a contiguous fp32 CUDA tensor [pages, kv_heads, page_size]")
     return t.data_ptr()
@@ -92,20 +115,21 @@ def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, table: torch.Tenso
     """Quantises k, v (bf16 or fp32 ``[rows, kv_heads, head_dim]``, any row and head strides of whole
     16 bytes) into the cache as the sequences' last tokens.  ``weights``: its entries of the new tokens
     become zero."""
-    _heads(k, "k", cache)
-    _heads(v, "v", cache)
-    if v.dtype is not k.dtype or v.shape != k.shape or k.shape[1] != cache.kv_heads:
+    rows, heads, k_row, k_head = _heads(k, "k", cache)
+    v_rows, v_heads, v_row, v_head = _heads(v, "v", cache)
+    dtype = k.dtype
+    if v.dtype is not dtype or v_rows != rows or heads != cache.kv_heads or v_heads != heads:
         raise ValueError("k and v must have one dtype and shape [rows, kv_heads, head_dim]")
-    if k.dtype is torch.bfloat16:
+    if dtype is _BF16:
         code = capi.OUT_BF16
-    elif k.dtype is torch.float32:
+    elif dtype is _F32:
         code = capi.OUT_F32
     else:
-        raise ValueError(f"k and v must be fp32 or bf16, not {k.dtype}")
-    b = _batch(table, lens, cu, k.shape[0], max_new)
+        raise ValueError(f"k and v must be fp32 or bf16, not {dtype}")
+    b = _batch(table, lens, cu, rows, max_new)
     wp = _weights_array(weights, "weights", cache) if weights is not None else None
-    capi.check(capi.lib().b2g_kv4_append(cache._args, b, k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1),
-                                         v.stride(0), v.stride(1), wp, _stream(stream)), "b2g_kv4_append")
+    capi.check(capi.lib().b2g_kv4_append(cache._args, b, k.data_ptr(), v.data_ptr(), code, k_row, k_head, v_row, v_head, wp,
+                                         _raw_stream(stream, k.device)), "b2g_kv4_append")
 
 
 def read(cache: KV4Cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor | None, rows: int,
@@ -113,10 +137,11 @@ def read(cache: KV4Cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Te
     """bf16 (k, v) ``[rows, kv_heads, head_dim]``: rows ``cu[b]:cu[b + 1]`` hold sequence b's tokens
     ``start[b]``, ``start[b] + 1``, ... as the cache has them."""
     b = _batch(table, None, cu, rows, None)
-    sp = _ints(start, "start", 1, b.seqs)
-    out = torch.empty((2, rows, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.k.device)
-    k, v = out.unbind(0)
-    capi.check(capi.lib().b2g_kv4_read(cache._args, b, sp, k.data_ptr(), v.data_ptr(), _stream(stream)), "b2g_kv4_read")
+    sp = _ints(start, "start", b.seqs)
+    shape = (rows, cache.kv_heads, cache.head_dim)
+    k, v = cache.k.new_empty(shape, dtype=_BF16), cache.k.new_empty(shape, dtype=_BF16)
+    capi.check(capi.lib().b2g_kv4_read(cache._args, b, sp, k.data_ptr(), v.data_ptr(), _raw_stream(stream, k.device)),
+               "b2g_kv4_read")
     return k, v
 
 
@@ -131,7 +156,7 @@ def workspace(cache: KV4Cache) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=cache.k.device)
 
 
-def _workspace(cache: KV4Cache, stream: int | None) -> torch.Tensor:
+def _workspace(cache: KV4Cache, stream: int) -> torch.Tensor:
     """The workspace this module keeps for a device, stream and head_dim."""
     key = (cache.k.device.index, stream, cache.head_dim)
     held = _WORKSPACES.get(key)
@@ -149,25 +174,24 @@ def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch
     (``causal``) and j > p - window (``window`` > 0); scores are ``scale * q . k`` (default
     head_dim ** -0.5), capped as ``softcap * tanh(s / softcap)``.  lse fp32 ``[rows, heads]`` is the
     logarithm of the sum of exp(scores); a query that sees nothing gives out 0 and lse -inf."""
-    _heads(q, "q", cache)
-    if q.dtype is not torch.bfloat16:
+    rows, heads, q_row, q_head = _heads(q, "q", cache)
+    if q.dtype is not _BF16:
         raise ValueError(f"q must be bf16, not {q.dtype}")
-    rows, heads = q.shape[0], q.shape[1]
     b = _batch(table, lens, cu, rows, max_q)
     if out is None:
-        out = torch.empty((rows, heads, cache.head_dim), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((rows, heads, cache.head_dim))
+        o_row, o_head = heads * cache.head_dim, cache.head_dim
     else:
-        _heads(out, "out", cache)
-        if out.dtype is not torch.bfloat16 or out.shape != q.shape:
+        o_rows, o_heads, o_row, o_head = _heads(out, "out", cache)
+        if out.dtype is not _BF16 or o_rows != rows or o_heads != heads:
             raise ValueError("out must be bf16 of q's shape")
-    lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device)
-    st = _stream(stream)
+    lse = q.new_empty((rows, heads), dtype=_F32)
+    st = _raw_stream(stream, q.device)
     if ws is None:
-        ws = _workspace(cache, st.value)
+        ws = _workspace(cache, st)
     mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
-    capi.check(capi.lib().b2g_kv4_attention(cache._args, b, mask, q.data_ptr(), q.stride(0), q.stride(1), heads,
-                                            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), ws.data_ptr(),
-                                            ws.numel(), st), "b2g_kv4_attention")
+    capi.check(capi.lib().b2g_kv4_attention(cache._args, b, mask, q.data_ptr(), q_row, q_head, heads, out.data_ptr(), o_row, o_head,
+                                            lse.data_ptr(), ws.data_ptr(), ws.numel(), st), "b2g_kv4_attention")
     return out, lse
 
 
@@ -178,18 +202,18 @@ def weights(q: torch.Tensor, lse: torch.Tensor, cache: KV4Cache, table: torch.Te
     """``gathered`` (fp32 ``[pages, kv_heads, page_size]``) plus, for each cached token of the batch, the
     attention weight exp(score - lse) summed over the sequence's query rows and the kv head's query heads;
     written to ``out`` (default: ``gathered`` itself).  q, lse and the mask as for :func:`attention`."""
-    _heads(q, "q", cache)
-    if q.dtype is not torch.bfloat16:
+    rows, heads, q_row, q_head = _heads(q, "q", cache)
+    if q.dtype is not _BF16:
         raise ValueError(f"q must be bf16, not {q.dtype}")
-    if lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2] or not lse.is_cuda:
+    if lse.dtype is not _F32 or not lse.is_contiguous() or lse.shape != (rows, heads) or not lse.is_cuda:
         raise ValueError("lse must be a contiguous fp32 CUDA tensor [rows, heads]")
-    out = gathered if out is None else out
-    b = _batch(table, lens, cu, q.shape[0], max_q)
+    wp = _weights_array(gathered, "gathered", cache)
+    op = wp if out is None else _weights_array(out, "out", cache)
+    b = _batch(table, lens, cu, rows, max_q)
     mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
-    capi.check(capi.lib().b2g_kv4_weights(cache._args, b, mask, q.data_ptr(), q.stride(0), q.stride(1), q.shape[1],
-                                          lse.data_ptr(), _weights_array(gathered, "gathered", cache),
-                                          _weights_array(out, "out", cache), _stream(stream)), "b2g_kv4_weights")
-    return out
+    capi.check(capi.lib().b2g_kv4_weights(cache._args, b, mask, q.data_ptr(), q_row, q_head, heads, lse.data_ptr(), wp, op,
+                                          _raw_stream(stream, q.device)), "b2g_kv4_weights")
+    return gathered if out is None else out
 
 
 def evict(cache: KV4Cache, gathered: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, budget: int, sink: int = 4,
@@ -201,12 +225,13 @@ def evict(cache: KV4Cache, gathered: torch.Tensor, table: torch.Tensor, lens: to
     weights with them.  kept: int32 ``[seqs, kv_heads, budget]``, the numbers they had, then -1;
     ``out_lens`` may be ``lens``."""
     b = _batch(table, lens, None, table.shape[0], None)
-    out_table = table if out_table is None else out_table
-    op = _ints(out_table, "out_table", 2, b.seqs)
+    op, out_seqs, out_width = (b.table, b.seqs, b.table_width) if out_table is None else _table(out_table, "out_table")
+    if out_seqs != b.seqs:
+        raise ValueError(f"out_table has {out_seqs} sequences, not {b.seqs}")
     if out_lens is None:
-        out_lens = torch.empty_like(lens)
-    kept = torch.empty((b.seqs, cache.kv_heads, max(budget, 0)), dtype=torch.int32, device=lens.device)
+        out_lens = lens.new_empty(lens.shape)
+    kept = lens.new_empty((b.seqs, cache.kv_heads, max(budget, 0)))
     capi.check(capi.lib().b2g_kv4_evict(cache._args, b, _weights_array(gathered, "gathered", cache), budget, sink, recent, op,
-                                        out_table.shape[1], kept.data_ptr(), _ints(out_lens, "out_lens", 1, b.seqs),
-                                        _stream(stream)), "b2g_kv4_evict")
+                                        out_width, kept.data_ptr(), _ints(out_lens, "out_lens", b.seqs),
+                                        _raw_stream(stream, lens.device)), "b2g_kv4_evict")
     return kept, out_lens
