@@ -81,51 +81,70 @@ __device__ __forceinline__ int kv4_scale_byte(float amax) {
   return min(max(byte, kKv4ScaleMin), kKv4ScaleMax);
 }
 
+// Tokens of a row-wise kernel: thread `in` of a row's per_row, over all rows.  A block of 256
+// threads has 256 / per_row rows at a time, or a row in several goes; all its threads take the same
+// number of steps, so that lanes can exchange.  f(row, in, live)
+template <typename F>
+__device__ __forceinline__ void kv4_for_rows(int rows, int per_row, F&& f) {
+  const int at_once = max(1, 256 / per_row);
+  const int sub = per_row < 256 ? static_cast<int>(threadIdx.x) / per_row : 0;
+  const int in0 = static_cast<int>(threadIdx.x) - sub * per_row;
+  for (long long row0 = static_cast<long long>(blockIdx.x) * at_once; row0 < rows; row0 += static_cast<long long>(gridDim.x) * at_once) {
+    const int row = static_cast<int>(row0) + sub;
+    const bool live = sub < at_once && row0 + sub < rows;
+    for (int in = in0; in - in0 < per_row; in += 256) f(live ? row : 0, live && in < per_row ? in : 0, live && in < per_row);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// append: one thread per 8 channels, four threads per scale block.  A row of a batch is
-// K and V of every head: 2 * heads * D / 8 threads, so a warp reads 512 consecutive bytes
-// (bf16) and writes 128.  Bound by the input's bytes (bf16: 4 of the 5.06 bytes moved per value pair).
+// append: one thread per 8 channels of a token's K and V, four threads per scale block, so a
+// warp reads 1 KB (bf16) and writes 256 bytes, and the walk from row to page is paid once for
+// both.  Bound by bytes: the input is 4 (bf16) or 8 (fp32) of 5.06 or 9.06 moved per value pair.
 // ---------------------------------------------------------------------------
 template <typename In, int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_append_kernel(Kv4Cache c, Kv4Batch bt, const In* __restrict__ k, const In* __restrict__ v, long long k_row,
                       long long k_head, long long v_row, long long v_head, float* __restrict__ weights,
                       int* status) {
-  constexpr int kPer = D / 8;  // threads of one head's K or V
-  const int per_row = 2 * c.heads * kPer;
-  const long long total = static_cast<long long>(bt.rows) * per_row;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i - (threadIdx.x & 31) < total; i += gridDim.x * 256ll) {
-    const bool live = i < total;
-    const int row = live ? static_cast<int>(i / per_row) : 0;
-    const int in = static_cast<int>(i - static_cast<long long>(row) * per_row);
-    const int hv = in / kPer, g = in % kPer;
-    const bool is_v = hv >= c.heads;
-    const int head = is_v ? hv - c.heads : hv;
-    float x[8] = {};
-    if (live) load8_f32((is_v ? v + row * v_row + head * v_head : k + row * k_row + head * k_head) + g * 8, x);
-    float amax = 0.f;
+  constexpr int kPer = D / 8;  // threads of one head
+  griddep_wait();
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
+    const int head = in / kPer, g = in % kPer;
+    float x[2][8] = {};
+    if (live) {
+      load8_f32(k + row * k_row + head * k_head + g * 8, x[0]);
+      load8_f32(v + row * v_row + head * v_head + g * 8, x[1]);
+    }
+    float amax[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    if (!live) continue;
+    for (int i = 0; i < 2; ++i) {
+      amax[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax[i] = fmaxf(amax[i], fabsf(x[i][j]));
+      amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1));
+      amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 2));
+    }
+    if (!live) return;
     const int b = kv4_seq_of_row(bt, row);
     int first, end;
     kv4_rows(bt, b, first, end);
     const int len = kv4_len(bt, b, c.page_log2);
     const int token = __ldg(bt.lens + b) - (end - row);
-    if (row < first || row >= end || token < 0 || token >= len) continue;
+    if (row < first || row >= end || token < 0 || token >= len) return;
     const long long at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, token, status);
-    if (at < 0) continue;
-    const int byte = kv4_scale_byte(amax);
-    const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
-    uint32_t pk = 0;
+    if (at < 0) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pk |= f32_to_e2m1(x[j] * inv) << (4 * j);
-    *reinterpret_cast<uint32_t*>((is_v ? c.v : c.k) + at * (D / 2) + g * 4) = pk;
-    if ((g & 3) == 0) (is_v ? c.vs : c.ks)[at * (D / 32) + (g >> 2)] = static_cast<uint8_t>(byte);
-    if (weights && !is_v && g == 0) weights[at] = 0.f;
-  }
+    for (int i = 0; i < 2; ++i) {
+      const int byte = kv4_scale_byte(amax[i]);
+      const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
+      uint32_t pk = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pk |= f32_to_e2m1(x[i][j] * inv) << (4 * j);
+      *reinterpret_cast<uint32_t*>((i ? c.v : c.k) + at * (D / 2) + g * 4) = pk;
+      if ((g & 3) == 0) (i ? c.vs : c.ks)[at * (D / 32) + (g >> 2)] = static_cast<uint8_t>(byte);
+    }
+    if (weights && g == 0) weights[at] = 0.f;
+  });
 }
 
 // Value of code `n` (its low four bits): 2^(e - 1) (1 + m / 2), or m / 2 for e = 0.
@@ -139,20 +158,17 @@ __device__ __forceinline__ float kv4_scale_value(int byte) {
   return __int_as_float(min(max(byte, kKv4ScaleMin), kKv4ScaleMax) << 23);
 }
 
-// read: one thread per 8 channels of K or V.  The output's bf16 values are the bound
-// (4 of 5.06 bytes per value pair).
+// read: one thread per 16 channels of a token's K and V.  The output's bf16 values are the
+// bound (4 of 5.06 bytes per value pair).
 template <int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_read_kernel(Kv4Cache c, Kv4Batch bt, const int* __restrict__ start, __nv_bfloat16* __restrict__ k,
                     __nv_bfloat16* __restrict__ v, int* status) {
-  constexpr int kPer = D / 8;
-  const long long per_kv = static_cast<long long>(bt.rows) * c.heads * kPer;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < 2 * per_kv; i += gridDim.x * 256ll) {
-    const bool is_v = i >= per_kv;
-    const long long o = is_v ? i - per_kv : i;
-    const int g = static_cast<int>(o % kPer);
-    const long long rh = o / kPer;
-    const int row = static_cast<int>(rh / c.heads), head = static_cast<int>(rh - static_cast<long long>(row) * c.heads);
+  constexpr int kPer = D / 16;
+  griddep_wait();
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
+    if (!live) return;
+    const int head = in / kPer, g = in % kPer;
     const int b = kv4_seq_of_row(bt, row);
     int first, end;
     kv4_rows(bt, b, first, end);
@@ -160,16 +176,28 @@ b2g_kv4_read_kernel(Kv4Cache c, Kv4Batch bt, const int* __restrict__ start, __nv
     long long at = -1;
     if (row >= first && row < end && token >= 0 && token < (static_cast<long long>(bt.width) << c.page_log2))
       at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, static_cast<int>(token), status);
-    uint32_t w[4] = {};
+    uint2 codes[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+    float s[2] = {0.f, 0.f};
     if (at >= 0) {
-      const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>((is_v ? c.v : c.k) + at * (D / 2)) + g);
-      const float s = kv4_scale_value(__ldg((is_v ? c.vs : c.ks) + at * (D / 32) + (g >> 2)));
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = pack_bf16x2(kv4_code_value(codes >> (8 * j)) * s, kv4_code_value(codes >> (8 * j + 4)) * s);
+      for (int i = 0; i < 2; ++i) {
+        codes[i] = *(reinterpret_cast<const uint2*>((i ? c.v : c.k) + at * (D / 2)) + g);
+        s[i] = kv4_scale_value((i ? c.vs : c.ks)[at * (D / 32) + (g >> 1)]);
+      }
     }
-    *reinterpret_cast<uint4*>((is_v ? v : k) + o * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4* to = reinterpret_cast<uint4*>((i ? v : k) + (static_cast<long long>(row) * c.heads + head) * D + g * 16);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t x = half ? codes[i].y : codes[i].x;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(kv4_code_value(x >> (8 * j)) * s[i], kv4_code_value(x >> (8 * j + 4)) * s[i]);
+        to[half] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -183,18 +211,24 @@ __device__ __forceinline__ uint32_t kv4_rank(float w) {
 }
 
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictHeld = 49152;  // ranks that fit in shared memory (192 KB)
 
 // One CTA per (sequence, kv head).  Radix selection over the weights of the tokens between
 // the first `sink` and the last `recent`: three passes of 11, 11 and 10 bits find the rank
-// `cut` of the last one kept and how many of that rank are, then a pass in token order
-// writes the kept numbers.
+// `cut` of the last one kept and how many of that rank are; then each warp, with a run of
+// consecutive tokens, counts and writes the kept numbers in order.  What it costs is latency:
+// kHeld: the ranks are read from memory once, four tokens a thread in flight, and kept in
+// shared memory; sequences that may be longer read them in every pass.
+template <bool kHeld>
 __global__ void __launch_bounds__(kEvictThreads)
 b2g_kv4_select_kernel(Kv4Cache c, Kv4Batch bt, const float* __restrict__ weights, int budget, int sink, int recent,
                       int* __restrict__ kept, int* status) {
+  extern __shared__ uint32_t held[];
   __shared__ int hist[2048];
-  __shared__ int warp_sum[32], warp_sum2[32];
+  __shared__ int warp_a[32], warp_b[32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
+  griddep_wait();
   const int h = blockIdx.x % c.heads, b = blockIdx.x / c.heads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = kv4_len(bt, b, c.page_log2);
@@ -205,23 +239,46 @@ b2g_kv4_select_kernel(Kv4Cache c, Kv4Batch bt, const float* __restrict__ weights
     return;
   }
   const int lo = sink, hi = len - recent;  // sink + recent <= budget < len
+  auto rank_at = [&](int j) {
+    const long long at = kv4_token(c, row, h, j, status);
+    return at < 0 ? 0u : kv4_rank(weights[at]);
+  };
+  auto rank = [&](int j) { return kHeld ? held[j - lo] : rank_at(j); };
+  if (kHeld) {
+    for (int j = lo + tid; j < hi; j += 4 * kEvictThreads) {
+      uint32_t r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = j + e * kEvictThreads < hi ? rank_at(j + e * kEvictThreads) : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e * kEvictThreads < hi) held[j + e * kEvictThreads - lo] = r[e];
+    }
+  }
+  // sum over the block's warps before this one, of a number each warp has
+  auto before = [&](int mine, int* sums) {
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    int x = lane < warp ? sums[lane] : 0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  };
+  const bool any = budget - sink - recent > 0;
   int need = budget - sink - recent;
   uint32_t prefix = 0;  // the bits of `cut` found so far
-  if (need > 0) {
+  if (any) {
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const int bits = pass == 2 ? 10 : 11;
       for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
       for (int j = lo + tid; j < hi; j += kEvictThreads) {
-        const long long at = kv4_token(c, row, h, j, status);
-        const uint32_t r = at < 0 ? 0u : kv4_rank(weights[at]);
+        const uint32_t r = rank(j);
         if (pass == 0 || (r >> (shift + bits)) == prefix) atomicAdd(&hist[(r >> shift) & ((1 << bits) - 1)], 1);
       }
       __syncthreads();
       // two bins a thread, from the top: how many lie above
-      const int n_bins = 1 << bits;
-      const int top = n_bins - 1 - 2 * tid;
+      const int top = (1 << bits) - 1 - 2 * tid;
       const int c0 = top >= 1 ? hist[top] : 0, c1 = top >= 1 ? hist[top - 1] : 0;
       int sum = c0 + c1;
 #pragma unroll
@@ -229,10 +286,7 @@ b2g_kv4_select_kernel(Kv4Cache c, Kv4Batch bt, const float* __restrict__ weights
         const int t = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += t;
       }
-      if (lane == 31) warp_sum[warp] = sum;
-      __syncthreads();
-      int above = sum - c0 - c1;
-      for (int w = 0; w < warp; ++w) above += warp_sum[w];
+      const int above = sum - c0 - c1 + before(__shfl_sync(0xffffffffu, sum, 31), warp_a);
       if (top >= 1) {
         if (above < need && above + c0 >= need) {
           s_prefix = (prefix << bits) | static_cast<uint32_t>(top);
@@ -248,45 +302,40 @@ b2g_kv4_select_kernel(Kv4Cache c, Kv4Batch bt, const float* __restrict__ weights
     }
   }
   const uint32_t cut = prefix;
-  const bool any = budget - sink - recent > 0;
-  // in token order: kept is what ranks above `cut`, and the first `need` of rank `cut`
-  int n_kept = 0, n_tied = 0;
-  for (int base = 0; base < len; base += kEvictThreads) {
-    const int j = base + tid;
-    bool keep = false, tied = false;
-    if (j < len) {
-      if (j < lo || j >= hi) {
-        keep = true;
-      } else if (any) {
-        const long long at = kv4_token(c, row, h, j, status);
-        const uint32_t r = at < 0 ? 0u : kv4_rank(weights[at]);
-        keep = r > cut;
-        tied = r == cut;
-      }
+  // a warp's run of tokens: kept is what ranks above `cut`, and the first `need` of rank `cut`
+  const int per = ((len + kEvictThreads - 1) / kEvictThreads) * 32;
+  const int t0 = min(warp * per, len), t1 = min(t0 + per, len);
+  auto classify = [&](int j, bool& keep, bool& tied) {
+    keep = tied = false;
+    if (j >= t1) return;
+    if (j < lo || j >= hi) {
+      keep = true;
+    } else if (any) {
+      const uint32_t r = rank(j);
+      keep = r > cut;
+      tied = r == cut;
     }
+  };
+  int n_keep = 0, n_tied = 0;
+  for (int j = t0 + lane; j - lane < t1; j += 32) {
+    bool keep, tied;
+    classify(j, keep, tied);
+    n_keep += __popc(__ballot_sync(0xffffffffu, keep));
+    n_tied += __popc(__ballot_sync(0xffffffffu, tied));
+  }
+  int ties = before(n_tied, warp_a);
+  __syncthreads();
+  int to = before(n_keep + max(0, min(n_tied, need - ties)), warp_b);
+  for (int j = t0 + lane; j - lane < t1; j += 32) {
+    bool keep, tied;
+    classify(j, keep, tied);
     const uint32_t below = (1u << lane) - 1u;
     const uint32_t tm = __ballot_sync(0xffffffffu, tied);
-    if (lane == 0) warp_sum2[warp] = __popc(tm);
-    __syncthreads();
-    int before = n_tied, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += warp_sum2[w];
-      all += warp_sum2[w];
-    }
-    n_tied += all;
-    if (tied && before + __popc(tm & below) < need) keep = true;
+    if (tied && ties + __popc(tm & below) < need) keep = true;
+    ties += __popc(tm);
     const uint32_t km = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) warp_sum[warp] = __popc(km);
-    __syncthreads();
-    int at_out = n_kept;
-    all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) at_out += warp_sum[w];
-      all += warp_sum[w];
-    }
-    n_kept += all;
-    if (keep) out[at_out + __popc(km & below)] = j;
-    __syncthreads();
+    if (keep) out[to + __popc(km & below)] = j;
+    to += __popc(km);
   }
 }
 
@@ -323,28 +372,52 @@ struct Kv4Piece {
   }
 };
 
-// To other pages: any order, one thread per piece.
+// To other pages, in any order: D / 16 lanes per token, a 16-byte piece each, the first lane
+// the scales and the weight too; a lane has four tokens in flight.
 template <int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_move_kernel(Kv4Cache c, Kv4Batch bt, float* weights, int budget, const int* __restrict__ out_table,
                     int out_width, const int* __restrict__ kept, int* new_lens, int* status) {
-  constexpr int kPieces = D / 16 + 1;
-  const long long total = static_cast<long long>(bt.seqs) * c.heads * budget * kPieces;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long t = i / kPieces;
-    const int piece = static_cast<int>(i - t * kPieces);
-    const long long bh = t / budget;
-    const int slot = static_cast<int>(t - bh * budget);
-    const int b = static_cast<int>(bh / c.heads), h = static_cast<int>(bh - static_cast<long long>(b) * c.heads);
-    if (slot == 0 && piece == 0 && h == 0) new_lens[b] = min(kv4_len(bt, b, c.page_log2), budget);
-    const int j = __ldg(kept + t);
-    if (j < 0) continue;
-    const long long from = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, h, j, status);
-    const long long to = kv4_token(c, out_table + static_cast<long long>(b) * out_width, h, slot, status);
-    if (from < 0 || to < 0) continue;
-    Kv4Piece<D> p;
-    p.load(c, weights, from, piece);
-    p.store(c, weights, to, piece);
+  constexpr int kLanes = D / 16, kTokens = 256 / kLanes, kDeep = 4;
+  griddep_wait();
+  const int h = blockIdx.y, b = blockIdx.z;
+  // lens may be new_lens: this thread alone reads and writes it
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) new_lens[b] = min(kv4_len(bt, b, c.page_log2), budget);
+  const int piece = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
+  const int* from_row = bt.table + static_cast<long long>(b) * bt.width;
+  const int* to_row = out_table + static_cast<long long>(b) * out_width;
+  const int* mine = kept + (static_cast<long long>(b) * c.heads + h) * budget;
+  for (int base = blockIdx.x * (kTokens * kDeep); base < budget; base += gridDim.x * (kTokens * kDeep)) {
+    int j[kDeep];
+    long long from[kDeep], to[kDeep];
+    Kv4Piece<D> p[kDeep], more[kDeep];
+#pragma unroll
+    for (int e = 0; e < kDeep; ++e) {
+      const int slot = base + e * kTokens + sub;
+      j[e] = slot < budget ? __ldg(mine + slot) : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kDeep; ++e) {
+      const int slot = base + e * kTokens + sub;
+      from[e] = to[e] = -1;
+      if (j[e] >= 0) {
+        from[e] = kv4_token(c, from_row, h, j[e], status);
+        to[e] = kv4_token(c, to_row, h, slot, status);
+      }
+      if (to[e] < 0) from[e] = -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kDeep; ++e)
+      if (from[e] >= 0) {
+        p[e].load(c, weights, from[e], piece);
+        if (piece == 0) more[e].load(c, weights, from[e], kLanes);
+      }
+#pragma unroll
+    for (int e = 0; e < kDeep; ++e)
+      if (from[e] >= 0) {
+        p[e].store(c, weights, to[e], piece);
+        if (piece == 0) more[e].store(c, weights, to[e], kLanes);
+      }
   }
 }
 
@@ -357,6 +430,7 @@ b2g_kv4_move_in_place_kernel(Kv4Cache c, Kv4Batch bt, float* weights, int budget
                              int* new_lens, int* status) {
   constexpr int kPieces = D / 16 + 1;
   constexpr int kTokens = 1024 / kPieces;
+  griddep_wait();
   const int h = blockIdx.x % c.heads, b = blockIdx.x / c.heads;
   const int* row = bt.table + static_cast<long long>(b) * bt.width;
   const int* mine = kept + (static_cast<long long>(b) * c.heads + h) * budget;

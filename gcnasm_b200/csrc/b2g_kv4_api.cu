@@ -20,13 +20,11 @@ namespace {
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-int launched() {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? B2G_OK : host_fail(B2G_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
-}
-
-int grid_for(long long threads, int block, int most) {
-  return static_cast<int>(std::max(1ll, std::min((threads + block - 1) / block, static_cast<long long>(most))));
+// Blocks of 256 threads for a row-wise kernel (kv4_for_rows): one each for the rows it has at
+// once, as many as are resident at most.
+int row_grid(long long rows, int per_row, int sms) {
+  const long long at_once = std::max(1, 256 / per_row);
+  return static_cast<int>(std::min((rows + at_once - 1) / at_once, 8ll * sms));
 }
 
 struct Call {
@@ -97,7 +95,10 @@ void by_dim(int dim, F&& f) {
   else f(std::integral_constant<int, 256>());
 }
 
-// A launch that may begin while the kernel before it ends (each kernel waits for that one first).
+// A launch that may begin when the blocks of the kernel before it have ended, before that kernel's
+// end has been made visible; each kernel here waits for that first.  Only the decode kernel lets its
+// follower begin earlier: what the others read and write in place (lens, weights) must not be
+// cached by a block of the follower's SM once the follower is there.
 template <typename... P, typename... A>
 int launch(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, A... args) {
   cudaLaunchAttribute attr[1];
@@ -135,7 +136,10 @@ template <typename K>
 int resident(K kernel, int block, size_t smem, int most, int dev, std::atomic<int> (&known)[64]) {
   int n = known[dev].load();
   if (n) return n;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024) != cudaSuccess ||
+  cudaFuncAttributes has{};
+  if (cudaFuncGetAttributes(&has, kernel) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(227 * 1024 - has.sharedSizeBytes)) != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, smem) != cudaSuccess) {
     (void)cudaGetLastError();
     return 0;
@@ -204,17 +208,15 @@ int b2g_kv4_append(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const
   if (rc) return rc;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const int grid = grid_for(static_cast<long long>(batch->rows) * 2 * f.c.heads * (D / 8), 256, 16 * f.sms);
+    const dim3 grid(row_grid(batch->rows, f.c.heads * (D / 8), f.sms));
     if (x_dtype == B2G_OUT_F32)
-      b2g_kv4_append_kernel<float, D><<<grid, 256, 0, f.st>>>(f.c, f.bt, static_cast<const float*>(k), static_cast<const float*>(v),
-                                                              k_row_stride, k_head_stride, v_row_stride, v_head_stride, weights,
-                                                              f.status);
+      rc = launch(b2g_kv4_append_kernel<float, D>, grid, 256, 0, f.st, f.c, f.bt, static_cast<const float*>(k),
+                  static_cast<const float*>(v), k_row_stride, k_head_stride, v_row_stride, v_head_stride, weights, f.status);
     else
-      b2g_kv4_append_kernel<__nv_bfloat16, D><<<grid, 256, 0, f.st>>>(
-          f.c, f.bt, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), k_row_stride, k_head_stride,
-          v_row_stride, v_head_stride, weights, f.status);
+      rc = launch(b2g_kv4_append_kernel<__nv_bfloat16, D>, grid, 256, 0, f.st, f.c, f.bt, static_cast<const __nv_bfloat16*>(k),
+                  static_cast<const __nv_bfloat16*>(v), k_row_stride, k_head_stride, v_row_stride, v_head_stride, weights, f.status);
   });
-  return launched();
+  return rc;
 }
 
 int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const int* start, void* k, void* v, void* stream) {
@@ -226,11 +228,10 @@ int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const i
   if (rc) return rc;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const int grid = grid_for(static_cast<long long>(batch->rows) * 2 * f.c.heads * (D / 8), 256, 16 * f.sms);
-    b2g_kv4_read_kernel<D><<<grid, 256, 0, f.st>>>(f.c, f.bt, start, static_cast<__nv_bfloat16*>(k),
-                                                   static_cast<__nv_bfloat16*>(v), f.status);
+    rc = launch(b2g_kv4_read_kernel<D>, dim3(row_grid(batch->rows, f.c.heads * (D / 16), f.sms)), 256, 0, f.st, f.c, f.bt, start,
+                static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), f.status);
   });
-  return launched();
+  return rc;
 }
 
 long long b2g_kv4_workspace_bytes(int head_dim) {
@@ -300,17 +301,27 @@ int b2g_kv4_evict(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, float*
       static_cast<long long>(out_width) * cache->page_size < std::min<long long>(budget, static_cast<long long>(batch->table_width) * cache->page_size))
     return host_fail(B2G_ERR_INVALID_ARG, "out_table of %d pages a sequence does not hold the budget of %d tokens", out_width, budget);
   const int lists = f.bt.seqs * f.c.heads;
-  b2g_kv4_select_kernel<<<lists, kEvictThreads, 0, f.st>>>(f.c, f.bt, weights, budget, sink, recent, kept, f.status);
-  if ((rc = launched())) return rc;
+  const long long longest = static_cast<long long>(f.bt.width) << f.c.page_log2;
+  if (longest <= kEvictHeld) {
+    static std::atomic<int> known[64];
+    if (resident(b2g_kv4_select_kernel<true>, kEvictThreads, kEvictHeld * 4, 2, f.dev, known) < 1)
+      return host_fail(B2G_ERR_CUDA, "the select kernel does not fit on the device");
+    rc = launch(b2g_kv4_select_kernel<true>, dim3(lists), kEvictThreads, longest * 4, f.st, f.c, f.bt, weights, budget, sink, recent,
+                kept, f.status);
+  } else {
+    rc = launch(b2g_kv4_select_kernel<false>, dim3(lists), kEvictThreads, 0, f.st, f.c, f.bt, weights, budget, sink, recent, kept,
+                f.status);
+  }
+  if (rc) return rc;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (in_place)
-      b2g_kv4_move_in_place_kernel<D><<<lists, 1024, 0, f.st>>>(f.c, f.bt, weights, budget, kept, new_lens, f.status);
+      rc = launch(b2g_kv4_move_in_place_kernel<D>, dim3(lists), 1024, 0, f.st, f.c, f.bt, weights, budget, kept, new_lens, f.status);
     else
-      b2g_kv4_move_kernel<D><<<grid_for(static_cast<long long>(lists) * budget * (D / 16 + 1), 256, 16 * f.sms), 256, 0, f.st>>>(
-          f.c, f.bt, weights, budget, out_table, out_width, kept, new_lens, f.status);
+      rc = launch(b2g_kv4_move_kernel<D>, dim3((budget + 16384 / D - 1) / (16384 / D), f.c.heads, f.bt.seqs), 256, 0, f.st, f.c, f.bt,
+                  weights, budget, out_table, out_width, kept, new_lens, f.status);
   });
-  return launched();
+  return rc;
 }
 
 }  // extern "C"

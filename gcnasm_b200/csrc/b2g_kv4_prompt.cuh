@@ -480,7 +480,6 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   __syncthreads();
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc<512>(tmem);
-  griddep_launch_dependents();
 }
 
 }  // namespace b2g

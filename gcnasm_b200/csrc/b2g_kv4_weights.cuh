@@ -186,7 +186,6 @@ b2g_kv4_weights_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, cons
         }
       }
   }
-  griddep_launch_dependents();
 }
 
 }  // namespace b2g
