@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <cstdint>
 #include <type_traits>
@@ -81,18 +82,29 @@ __device__ __forceinline__ int kv4_scale_byte(float amax) {
   return min(max(byte, kKv4ScaleMin), kKv4ScaleMax);
 }
 
+constexpr int kRowsDeep = 2;
+
 // Tokens of a row-wise kernel: thread `in` of a row's per_row, over all rows.  A block of 256
-// threads has 256 / per_row rows at a time, or a row in several goes; all its threads take the same
-// number of steps, so that lanes can exchange.  f(row, in, live)
+// threads has 256 / per_row rows at a time, or a row in several goes, and takes kRowsDeep of such
+// steps together so that as many walks from row to page are under way; all its threads take the
+// same number of steps, so that lanes can exchange.  f(rows, in, live), a row each of the steps.
 template <typename F>
 __device__ __forceinline__ void kv4_for_rows(int rows, int per_row, F&& f) {
   const int at_once = max(1, 256 / per_row);
   const int sub = per_row < 256 ? static_cast<int>(threadIdx.x) / per_row : 0;
   const int in0 = static_cast<int>(threadIdx.x) - sub * per_row;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * at_once; row0 < rows; row0 += static_cast<long long>(gridDim.x) * at_once) {
-    const int row = static_cast<int>(row0) + sub;
-    const bool live = sub < at_once && row0 + sub < rows;
-    for (int in = in0; in - in0 < per_row; in += 256) f(live ? row : 0, live && in < per_row ? in : 0, live && in < per_row);
+  const long long step = static_cast<long long>(gridDim.x) * at_once;
+  for (long long row0 = static_cast<long long>(blockIdx.x) * at_once; row0 < rows; row0 += kRowsDeep * step) {
+    for (int in = in0; in - in0 < per_row; in += 256) {
+      int row[kRowsDeep];
+      bool live[kRowsDeep];
+#pragma unroll
+      for (int i = 0; i < kRowsDeep; ++i) {
+        live[i] = sub < at_once && row0 + i * step + sub < rows && in < per_row;
+        row[i] = live[i] ? static_cast<int>(row0 + i * step) + sub : 0;
+      }
+      f(row, in < per_row ? in : 0, live);
+    }
   }
 }
 
@@ -108,93 +120,121 @@ b2g_kv4_append_kernel(Kv4Cache c, Kv4Batch bt, const In* __restrict__ k, const I
                       int* status) {
   constexpr int kPer = D / 8;  // threads of one head
   griddep_wait();
-  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](const int (&row)[kRowsDeep], int in, const bool (&live)[kRowsDeep]) {
     const int head = in / kPer, g = in % kPer;
-    float x[2][8] = {};
-    if (live) {
-      load8_f32(k + row * k_row + head * k_head + g * 8, x[0]);
-      load8_f32(v + row * v_row + head * v_head + g * 8, x[1]);
+    float x[kRowsDeep][2][8] = {};
+#pragma unroll
+    for (int n = 0; n < kRowsDeep; ++n)
+      if (live[n]) {
+        load8_f32(k + row[n] * k_row + head * k_head + g * 8, x[n][0]);
+        load8_f32(v + row[n] * v_row + head * v_head + g * 8, x[n][1]);
+      }
+    long long at[kRowsDeep];
+#pragma unroll
+    for (int n = 0; n < kRowsDeep; ++n) {
+      at[n] = -1;
+      if (live[n]) {
+        const int b = kv4_seq_of_row(bt, row[n]);
+        int first, end;
+        kv4_rows(bt, b, first, end);
+        const int len = kv4_len(bt, b, c.page_log2);
+        const int token = __ldg(bt.lens + b) - (end - row[n]);
+        if (row[n] >= first && row[n] < end && token >= 0 && token < len)
+          at[n] = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, token, status);
+      }
     }
-    float amax[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      amax[i] = 0.f;
+    for (int n = 0; n < kRowsDeep; ++n) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax[i] = fmaxf(amax[i], fabsf(x[i][j]));
-      amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1));
-      amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 2));
+      for (int i = 0; i < 2; ++i) {
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[n][i][j]));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        if (at[n] < 0) continue;
+        const int byte = kv4_scale_byte(amax);
+        const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
+        uint32_t pk = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pk |= f32_to_e2m1(x[n][i][j] * inv) << (4 * j);
+        *reinterpret_cast<uint32_t*>((i ? c.v : c.k) + at[n] * (D / 2) + g * 4) = pk;
+        if ((g & 3) == 0) (i ? c.vs : c.ks)[at[n] * (D / 32) + (g >> 2)] = static_cast<uint8_t>(byte);
+      }
+      if (at[n] >= 0 && weights && g == 0) weights[at[n]] = 0.f;
     }
-    if (!live) return;
-    const int b = kv4_seq_of_row(bt, row);
-    int first, end;
-    kv4_rows(bt, b, first, end);
-    const int len = kv4_len(bt, b, c.page_log2);
-    const int token = __ldg(bt.lens + b) - (end - row);
-    if (row < first || row >= end || token < 0 || token >= len) return;
-    const long long at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, token, status);
-    if (at < 0) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int byte = kv4_scale_byte(amax[i]);
-      const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
-      uint32_t pk = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pk |= f32_to_e2m1(x[i][j] * inv) << (4 * j);
-      *reinterpret_cast<uint32_t*>((i ? c.v : c.k) + at * (D / 2) + g * 4) = pk;
-      if ((g & 3) == 0) (i ? c.vs : c.ks)[at * (D / 32) + (g >> 2)] = static_cast<uint8_t>(byte);
-    }
-    if (weights && g == 0) weights[at] = 0.f;
   });
 }
 
-// Value of code `n` (its low four bits): 2^(e - 1) (1 + m / 2), or m / 2 for e = 0.
-__device__ __forceinline__ float kv4_code_value(uint32_t n) {
-  // e and m placed as an fp32 exponent and top mantissa bit: the value times 2^-126 (a
-  // subnormal for e = 0), which the multiplication makes exact and normal again
-  return __uint_as_float(((n & 8u) << 28) | ((n & 7u) << 22)) * __int_as_float((126 + 127) << 23);
+// The four bytes of w, two E2M1 codes each, as f16 pairs (low code in the low half).
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
 }
 
 __device__ __forceinline__ float kv4_scale_value(int byte) {
   return __int_as_float(min(max(byte, kKv4ScaleMin), kKv4ScaleMax) << 23);
 }
 
-// read: one thread per 16 channels of a token's K and V.  The output's bf16 values are the
-// bound (4 of 5.06 bytes per value pair).
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// read: one thread per 16 channels of a token's K and V, each written as one 32-byte sector.
+// The output's bf16 values are the bound (4 of 5.06 bytes per value pair).
 template <int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_read_kernel(Kv4Cache c, Kv4Batch bt, const int* __restrict__ start, __nv_bfloat16* __restrict__ k,
                     __nv_bfloat16* __restrict__ v, int* status) {
   constexpr int kPer = D / 16;
   griddep_wait();
-  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
-    if (!live) return;
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](const int (&row)[kRowsDeep], int in, const bool (&live)[kRowsDeep]) {
     const int head = in / kPer, g = in % kPer;
-    const int b = kv4_seq_of_row(bt, row);
-    int first, end;
-    kv4_rows(bt, b, first, end);
-    const long long token = static_cast<long long>(__ldg(start + b)) + row - first;
-    long long at = -1;
-    if (row >= first && row < end && token >= 0 && token < (static_cast<long long>(bt.width) << c.page_log2))
-      at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, static_cast<int>(token), status);
-    uint2 codes[2] = {make_uint2(0, 0), make_uint2(0, 0)};
-    float s[2] = {0.f, 0.f};
-    if (at >= 0) {
+    long long at[kRowsDeep];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        codes[i] = *(reinterpret_cast<const uint2*>((i ? c.v : c.k) + at * (D / 2)) + g);
-        s[i] = kv4_scale_value((i ? c.vs : c.ks)[at * (D / 32) + (g >> 1)]);
+    for (int n = 0; n < kRowsDeep; ++n) {
+      at[n] = -1;
+      if (live[n]) {
+        const int b = kv4_seq_of_row(bt, row[n]);
+        int first, end;
+        kv4_rows(bt, b, first, end);
+        const long long token = static_cast<long long>(__ldg(start + b)) + row[n] - first;
+        if (row[n] >= first && row[n] < end && token >= 0 && token < (static_cast<long long>(bt.width) << c.page_log2))
+          at[n] = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, static_cast<int>(token), status);
       }
     }
+    uint2 codes[kRowsDeep][2];
+    float s[kRowsDeep][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint4* to = reinterpret_cast<uint4*>((i ? v : k) + (static_cast<long long>(row) * c.heads + head) * D + g * 16);
+    for (int n = 0; n < kRowsDeep; ++n)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t x = half ? codes[i].y : codes[i].x;
-        uint32_t w[4];
+      for (int i = 0; i < 2; ++i) {
+        codes[n][i] = make_uint2(0, 0);
+        s[n][i] = 0.f;
+        if (at[n] >= 0) {
+          codes[n][i] = *(reinterpret_cast<const uint2*>((i ? c.v : c.k) + at[n] * (D / 2)) + g);
+          s[n][i] = kv4_scale_value((i ? c.vs : c.ks)[at[n] * (D / 32) + (g >> 1)]);
+        }
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(kv4_code_value(x >> (8 * j)) * s[i], kv4_code_value(x >> (8 * j + 4)) * s[i]);
-        to[half] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int n = 0; n < kRowsDeep; ++n) {
+      if (!live[n]) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t w[8], x[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j % 4 == 0) e2m1x8_to_f16(j ? codes[n][i].y : codes[n][i].x, x);
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x[j % 4]));
+          w[j] = pack_bf16x2(y.x * s[n][i], y.y * s[n][i]);
+        }
+        st_global_v8((i ? v : k) + (static_cast<long long>(row[n]) * c.heads + head) * D + g * 16, w);
       }
     }
   });

@@ -122,16 +122,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 
-// The four bytes of w, two E2M1 codes each, as f16 pairs (low code in the low half).
-__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "mov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
-}
-
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -694,14 +684,12 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   griddep_launch_dependents();
 }
 
-// Joins the parts of an item that was cut: CTA i has the item that decode CTA i began.  512
-// threads: the warps share the item's rows and, where there are fewer rows than warps, its parts.
+// Joins the parts of an item that was cut: block (i, y) has rows 4 y .. 4 y + 3 of the item that
+// decode CTA i began.  512 threads: four warps share a row's parts, eight in flight each.
 template <int D, int NT>
 __global__ void __launch_bounds__(512)
-b2g_kv4_join_kernel(Kv4Cache c, Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial,
-                    const int4* __restrict__ desc) {
-  constexpr int kRows = 8 * NT, kE = D / 32;
-  constexpr int kShare = kRows >= 16 ? 1 : 16 / kRows;  // warps to a row
+b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial, const int4* __restrict__ desc) {
+  constexpr int kRows = 8 * NT, kE = D / 32, kShare = 4;
   __shared__ float s_o[16][D];
   __shared__ float s_m[16], s_l[16];
   griddep_wait();
@@ -713,81 +701,73 @@ b2g_kv4_join_kernel(Kv4Cache c, Kv4Batch bt, Kv4Queries q, Kv4Out out, const flo
   const int blocks = (group_rows + kRows - 1) / kRows;
   const int h = d.z / blocks, r0 = (d.z - h * blocks) * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = warp % kShare;
-  for (int r = warp / kShare; r < kRows; r += 16 / kShare) {
-    float top = -INFINITY, sum = 0.f, o[kE] = {};
-    if (r0 + r < group_rows) {
-      auto slot_of = [&](int i) { return partial + (2ll * (blockIdx.x + i) + (i == 0 ? d.w : 0)) * (kRows * (D + 2)); };
+  const int share = warp % kShare, r = blockIdx.y * 4 + warp / kShare;
+  float top = -INFINITY, sum = 0.f, o[kE] = {};
+  // a part without a maximum weighs nothing, unless none has one: then sums that are NaN come through
+  auto weight = [](float m, float t) { return m == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(m - t); };
+  if (r0 + r < group_rows) {
 #pragma unroll 1
-      for (int i0 = share; i0 < d.x; i0 += 8 * kShare) {
-        float mm[8], ll[8], x[8][kE];
+    for (int i0 = share; i0 < d.x; i0 += 8 * kShare) {
+      float mm[8], ll[8], x[8][kE];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int i = i0 + j * kShare;
-          mm[j] = -INFINITY;
-          ll[j] = 0.f;
-          if (i < d.x) {
-            const float* s = slot_of(i);
-            mm[j] = s[kRows * D + 2 * r];
-            ll[j] = s[kRows * D + 2 * r + 1];
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * kShare;
+        mm[j] = -INFINITY;
+        ll[j] = 0.f;
 #pragma unroll
-            for (int e = 0; e < kE; e += 2) {
-              const float2 v = *reinterpret_cast<const float2*>(s + r * D + e * 32 + 2 * lane);
-              x[j][e] = v.x;
-              x[j][e + 1] = v.y;
-            }
-          } else {
+        for (int e = 0; e < kE; ++e) x[j][e] = 0.f;
+        if (i < d.x) {
+          const float* s = partial + (2ll * (blockIdx.x + i) + (i == 0 ? d.w : 0)) * (kRows * (D + 2));
+          mm[j] = s[kRows * D + 2 * r];
+          ll[j] = s[kRows * D + 2 * r + 1];
 #pragma unroll
-            for (int e = 0; e < kE; ++e) x[j][e] = 0.f;
+          for (int e = 0; e < kE; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(s + r * D + e * 32 + 2 * lane);
+            x[j][e] = v.x;
+            x[j][e + 1] = v.y;
           }
         }
-        float t = top;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t = fmaxf(t, mm[j]);
-        const float f = top == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(top - t);
-        sum *= f;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) o[e] *= f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float g = mm[j] == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(mm[j] - t);
-          sum += g * ll[j];
-#pragma unroll
-          for (int e = 0; e < kE; ++e) o[e] += g * x[j][e];
-        }
-        top = t;
       }
-    }
-    if (kShare > 1) {
+      float t = top;
 #pragma unroll
-      for (int e = 0; e < kE; e += 2)
-        *reinterpret_cast<float2*>(&s_o[warp][e * 32 + 2 * lane]) = make_float2(o[e], o[e + 1]);
-      if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
-      __syncthreads();
-      if (share == 0) {
-        float t = top;
-        for (int w = 1; w < kShare; ++w) t = fmaxf(t, s_m[warp + w]);
-        const float f = top == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(top - t);
-        sum *= f;
+      for (int j = 0; j < 8; ++j) t = fmaxf(t, mm[j]);
+      const float f = weight(top, t);
+      sum *= f;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) o[e] *= f;
-        for (int w = 1; w < kShare; ++w) {
-          const float mw = s_m[warp + w];
-          const float g = mw == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(mw - t);
-          sum += g * s_l[warp + w];
+      for (int e = 0; e < kE; ++e) o[e] *= f;
 #pragma unroll
-          for (int e = 0; e < kE; ++e) o[e] += g * s_o[warp + w][(e & ~1) * 32 + 2 * lane + (e & 1)];
-        }
-        top = t;
+      for (int j = 0; j < 8; ++j) {
+        const float g = weight(mm[j], t);
+        sum += g * ll[j];
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] += g * x[j][e];
       }
-    }
-    if (share == 0 && r0 + r < group_rows) {
-      const long long row = first + (r0 + r) / q.group;
-      const int head = h * q.group + (r0 + r) % q.group;
-#pragma unroll
-      for (int e = 0; e < kE; e += 2) kv4_finish(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), top, sum);
+      top = t;
     }
   }
+#pragma unroll
+  for (int e = 0; e < kE; e += 2) *reinterpret_cast<float2*>(&s_o[warp][e * 32 + 2 * lane]) = make_float2(o[e], o[e + 1]);
+  if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
+  __syncthreads();
+  if (share != 0 || r0 + r >= group_rows) return;
+  float t = top;
+#pragma unroll
+  for (int w = 1; w < kShare; ++w) t = fmaxf(t, s_m[warp + w]);
+  const float f = weight(top, t);
+  sum *= f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) o[e] *= f;
+#pragma unroll
+  for (int w = 1; w < kShare; ++w) {
+    const float g = weight(s_m[warp + w], t);
+    sum += g * s_l[warp + w];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] += g * s_o[warp + w][(e & ~1) * 32 + 2 * lane + (e & 1)];
+  }
+  const long long row = first + (r0 + r) / q.group;
+  const int head = h * q.group + (r0 + r) % q.group;
+#pragma unroll
+  for (int e = 0; e < kE; e += 2) kv4_finish(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), t, sum);
 }
 
 }  // namespace b2g
