@@ -166,16 +166,16 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   return launch(b2g_kv4_join_kernel<D, NT>, dim3(grid, 2 * NT), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
-template <int D>
+template <int D, bool kCap>
 int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, long long group_rows) {
   using Cfg = PromptCfg<D>;
   static std::atomic<int> known[64];
-  if (resident(b2g_kv4_prompt_kernel<D>, Cfg::kThreads, Cfg::kSmem, 1, f.dev, known) < 1)
+  if (resident(b2g_kv4_prompt_kernel<D, kCap>, Cfg::kThreads, Cfg::kSmem, 1, f.dev, known) < 1)
     return host_fail(B2G_ERR_CUDA, "the prompt kernel does not fit on the device");
   const long long blocks = (group_rows + Cfg::kRows - 1) / Cfg::kRows;
   if (blocks > 65535) return host_fail(B2G_ERR_UNSUPPORTED, "max_new %lld x the heads of a group is beyond %d rows", group_rows, 65535 * Cfg::kRows);
-  return launch(b2g_kv4_prompt_kernel<D>, dim3(f.c.heads, f.bt.seqs, static_cast<unsigned>(blocks)), Cfg::kThreads, Cfg::kSmem, f.st,
-                f.c, f.bt, m, q, o, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
+  return launch(b2g_kv4_prompt_kernel<D, kCap>, dim3(f.c.heads, f.bt.seqs, static_cast<unsigned>(blocks)), Cfg::kThreads, Cfg::kSmem,
+                f.st, f.c, f.bt, m, q, o, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
 }
 
 template <int D>
@@ -261,7 +261,7 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   const long long rows = static_cast<long long>(std::max(1, batch->cu ? std::min(batch->max_new, batch->rows) : 1)) * qs.group;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (rows >= kPromptRows) rc = prompt<D>(f, m, qs, o, rows);
+    if (rows >= kPromptRows) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, rows) : prompt<D, false>(f, m, qs, o, rows);
     else if (rows <= 8) rc = decode<D, 1>(f, m, qs, o, workspace);
     else if (rows <= 16 || D == 256) rc = decode<D, 2>(f, m, qs, o, workspace);
     else if constexpr (D < 256) rc = decode<D, 4>(f, m, qs, o, workspace);

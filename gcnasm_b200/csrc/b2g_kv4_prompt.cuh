@@ -103,6 +103,47 @@ __device__ __forceinline__ void sub2(float& a0, float& a1, float b0, float b1) {
       : "f"(b0), "f"(b1));
 }
 
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+// (a0, a1) = (a0 * b0 + c0, a1 * b1 + c1)
+__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
+// tanh x for |x| < 0.4 by the odd series (as kv4_cap), and by 1 - 2 / (e^2x + 1): to 2^-22
+// absolutely, exact at both ends.  The series takes no special function, which bound the kernel.
+__device__ __forceinline__ float kv4_tanh_near(float x) {
+  const float y = x * x;
+  float p = fmaf(y, -1382.f / 155925.f, 62.f / 2835.f);
+  p = fmaf(y, p, -17.f / 315.f);
+  p = fmaf(y, p, 2.f / 15.f);
+  p = fmaf(y, p, -1.f / 3.f);
+  return fmaf(x * y, p, x);
+}
+__device__ __forceinline__ void kv4_tanh_near2(float& x0, float& x1) {
+  float y0 = x0, y1 = x1, p0 = -1382.f / 155925.f, p1 = p0;
+  mul2(y0, y1, x0, x1);
+  fma2(p0, p1, y0, y1, 62.f / 2835.f, 62.f / 2835.f);
+  fma2(p0, p1, y0, y1, -17.f / 315.f, -17.f / 315.f);
+  fma2(p0, p1, y0, y1, 2.f / 15.f, 2.f / 15.f);
+  fma2(p0, p1, y0, y1, -1.f / 3.f, -1.f / 3.f);
+  mul2(y0, y1, x0, x1);
+  fma2(p0, p1, y0, y1, x0, x1);
+  x0 = p0, x1 = p1;
+}
+__device__ __forceinline__ float kv4_tanh_far(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(x * (2.f * kLog2e)) + 1.f));
+  return fmaf(r, -2.f, 1.f);
+}
+
 // bits [a, b) of a word
 __device__ __forceinline__ uint32_t kv4_bits(int a, int b) {
   a = min(max(a, 0), 32);
@@ -112,7 +153,7 @@ __device__ __forceinline__ uint32_t kv4_bits(int a, int b) {
   return below_b & ~below_a;
 }
 
-template <int D>
+template <int D, bool kCap>
 __global__ void __launch_bounds__(PromptCfg<D>::kThreads, 1)
 b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, uint64_t timeout_ns, int* status) {
   using Cfg = PromptCfg<D>;
@@ -200,9 +241,8 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     int lo, hi;
     kv4_visible(mask, len - rows + r / q.group, len, lo, hi);
     const float scale = fabsf(mask.scale) * kTwo64;
-    const bool cap = mask.softcap > 0.f;
-    const float cap_k = cap ? 2.f * kLog2e / mask.softcap : 0.f;
-    const float s_scale = cap ? scale : scale * kLog2e;
+    const float s_scale = kCap ? scale / mask.softcap : scale * kLog2e;  // a cap: tanh's argument
+    const float cap2 = kCap ? mask.softcap * kLog2e : 0.f;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     float m = -1e30f, l0 = 0.f, l1 = 0.f;
     bool ok = true;
@@ -230,28 +270,34 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         const uint32_t pages16 = ((there >> (col >> 4)) & 1u ? 0xFFFFu : 0u) | ((there >> ((col >> 4) + 1)) & 1u ? 0xFFFF0000u : 0u);
         return kv4_bits(lo - tb - col, hi - tb - col) & pages16;
       };
-      float top = -INFINITY;
-#pragma unroll
-      for (int col = 0; col < kN; col += 32) {
-        uint32_t x[32];
-        tmem_ld_32x32b_x32(s_at + col, x);
+      // the loops over S stay loops: three kinds of warps share the instruction cache
+      float top = -INFINITY, far = 0.f;
+#pragma unroll 1
+      for (int col = 0; col < kN; col += 64) {
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(s_at + col, x[0]);
+        tmem_ld_32x32b_x32(s_at + col + 32, x[1]);
         tc_wait_ld();
+        float t[4] = {top, top, top, top};
         if (masked) {
-          const uint32_t bits = seen(col);
+          const uint32_t bits[2] = {seen(col), seen(col + 32)};
 #pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, (bits >> e) & 1u ? __uint_as_float(x[e]) : -INFINITY);
-        } else {
-          float t1 = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            top = fmaxf(top, __uint_as_float(x[e]));
-            t1 = fmaxf(t1, __uint_as_float(x[e + 1]));
+          for (int e = 0; e < 64; ++e) {
+            if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e >> 5][e & 31])));
+            t[e & 3] = fmaxf(t[e & 3], (bits[e >> 5] >> (e & 31)) & 1u ? __uint_as_float(x[e >> 5][e & 31]) : -INFINITY);
           }
-          top = fmaxf(top, t1);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e >> 5][e & 31])));
+            t[e & 3] = fmaxf(t[e & 3], __uint_as_float(x[e >> 5][e & 31]));
+          }
         }
+        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       }
       top *= s_scale;  // s_scale is not negative; -inf x 0 is not a number, and no maximum
-      if (cap) top = kv4_cap(top, mask.softcap, cap_k) * kLog2e;
+      const bool near = kCap && __all_sync(0xffffffffu, far * s_scale < 0.4f);  // the series serves (a NaN is not near)
+      if (kCap) top = cap2 * (near ? kv4_tanh_near(top) : kv4_tanh_far(top));
       const bool grow = top > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow ? ex2(m - top) : 1.f;
@@ -263,7 +309,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
           // come before, but after step i - 2's, so the barrier is in phase i - 1 or just past it
           if (kSB == 2 && !(ok = wait(&o_done[tile], (i - 1) & 1))) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int col = 0; col < D; col += 32) {
             uint32_t x[32];
             tmem_ld_32x32b_x32(o_at + col, x);
@@ -274,20 +320,29 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
           }
         }
       }
-#pragma unroll
+#pragma unroll 1
       for (int col = 0; col < kN; col += 32) {
         uint32_t x[32], p[32];
         tmem_ld_32x32b_x32(s_at + col, x);
         tc_wait_ld();
+        if (kCap) {
+          if (near) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
+              mul2(y0, y1, s_scale, s_scale);
+              kv4_tanh_near2(y0, y1);
+              x[e] = __float_as_uint(y0), x[e + 1] = __float_as_uint(y1);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(kv4_tanh_far(__uint_as_float(x[e]) * s_scale));
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
-          if (cap) {
-            y0 = fmaf(kv4_cap(y0 * s_scale, mask.softcap, cap_k), kLog2e, -m);
-            y1 = fmaf(kv4_cap(y1 * s_scale, mask.softcap, cap_k), kLog2e, -m);
-          } else {
-            fma2(y0, y1, s_scale, -m);
-          }
+          fma2(y0, y1, kCap ? cap2 : s_scale, -m);
           x[e] = __float_as_uint(ex2(y0));
           x[e + 1] = __float_as_uint(ex2(y1));
         }
@@ -338,78 +393,70 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     }
   } else if (warp < kMmaWarp) {
     // ---------------------------------------------------------------- codes to bf16 tiles
-    constexpr int kWords = D == 64 ? 8 : 16;  // a thread's words of K, and of V, of a step
+    // K of a step, then V, by the same code: halves are fetched one ahead, page numbers a step ahead
+    constexpr int kWords = D == 64 ? 8 : 16;  // a thread's words of a half
     constexpr int kPer = D == 256 ? 2 : 1;    // threads to a token
     const int dt = threadIdx.x - kDecodeWarp * 32, tok = dt / kPer, part = dt % kPer;
     auto page_of = [&](int i) {
       const int token = (j0 + i) * kN + tok;
       return i < steps && token < len ? __ldg(pages + (token >> c.page_log2)) : -2;
     };
-    struct Raw {
-      uint4 k[kWords / 4], v[kWords / 4];
-      uint32_t ks, vs;
-    };
-    auto fetch = [&](Raw& x, int i, int page) {
+    // a step's token among all, -1 where it is not there
+    auto token_of = [&](int i, int page) {
       const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
       if (!there && page != -2) atomicCAS(status, 0, kDevBadPage);
       const int token = (j0 + i) * kN + tok;
-      const long long at = there ? ((static_cast<long long>(page) * c.heads + h) << c.page_log2) + (token & ((1 << c.page_log2) - 1)) : 0;
-#pragma unroll
-      for (int n = 0; n < kWords / 4; ++n) {
-        x.k[n] = x.v[n] = make_uint4(0, 0, 0, 0);
-        if (there) {
-          x.k[n] = __ldg(reinterpret_cast<const uint4*>(c.k + at * (D / 2) + part * 64) + n);
-          x.v[n] = __ldg(reinterpret_cast<const uint4*>(c.v + at * (D / 2) + part * 64) + n);
-        }
-      }
-      x.ks = x.vs = 0;
-      if (there) {
-        if constexpr (D == 64) {
-          x.ks = __ldg(reinterpret_cast<const uint16_t*>(c.ks + at * 2));
-          x.vs = __ldg(reinterpret_cast<const uint16_t*>(c.vs + at * 2));
-        } else {
-          x.ks = __ldg(reinterpret_cast<const uint32_t*>(c.ks + at * (D / 32)) + part);
-          x.vs = __ldg(reinterpret_cast<const uint32_t*>(c.vs + at * (D / 32)) + part);
-        }
-      }
+      return there ? ((static_cast<long long>(page) * c.heads + h) << c.page_log2) + (token & ((1 << c.page_log2) - 1)) : -1ll;
     };
-    // a thread's channels of one token: words of eight codes to 16-byte pieces of 128-byte swizzled rows
-    auto store = [&](uint8_t* tile, const uint4 (&x)[kWords / 4], uint32_t scales) {
+    auto fetch = [&](uint4 (&x)[kWords / 4], uint32_t& scales, const uint8_t* codes, const uint8_t* bytes, long long at) {
+      scales = 0;
+#pragma unroll
+      for (int n = 0; n < kWords / 4; ++n) x[n] = make_uint4(0, 0, 0, 0);
+      if (at < 0) return;
+#pragma unroll
+      for (int n = 0; n < kWords / 4; ++n) x[n] = *(reinterpret_cast<const uint4*>(codes + at * (D / 2) + part * 64) + n);
+      if constexpr (D == 64) scales = *reinterpret_cast<const uint16_t*>(bytes + at * 2);
+      else scales = *(reinterpret_cast<const uint32_t*>(bytes + at * (D / 32)) + part);
+    };
+    bool ok = true;
+    uint4 now[kWords / 4], next[kWords / 4];
+    uint32_t now_s, next_s;
+    int page = page_of(0);
+    long long at = steps > 0 ? token_of(0, page) : -1;
+    fetch(now, now_s, c.k, c.ks, at);
+    page = page_of(1);
+#pragma unroll 1
+    for (int i2 = 0; i2 < 2 * steps && ok; ++i2) {
+      const int i = i2 >> 1, st = i & 1;
+      const bool is_v = i2 & 1;
+      if (is_v) {
+        at = i + 1 < steps ? token_of(i + 1, page) : -1;
+        page = page_of(i + 2);
+      }
+      fetch(next, next_s, is_v ? c.k : c.v, is_v ? c.ks : c.vs, at);
+      uint64_t* empty = is_v ? &v_empty[st] : &k_empty[st];
+      if (!mbar_wait(empty, ((i >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
+      // a thread's channels of one token: words of eight codes to 16-byte pieces of 128-byte swizzled rows
+      uint8_t* tile = smem + (is_v ? Cfg::kOffV : Cfg::kOffK) + st * Cfg::kKBytes + tok * 128;
       uint32_t even, odd;
-      kv4_scales_bf16<62>(scales, even, odd);
+      kv4_scales_bf16<62>(now_s, even, odd);
 #pragma unroll
       for (int n = 0; n < kWords / 4; ++n) {
-        const uint32_t f16 = n == 0 ? even & 0xFFFFu : n == 1 ? odd & 0xFFFFu : n == 2 ? even >> 16 : odd >> 16;
-        const uint32_t f = f16 * 0x10001u;
-        const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+        const uint32_t f = __byte_perm(n & 1 ? odd : even, 0, n & 2 ? 0x3232 : 0x1010);
+        const uint32_t w[4] = {now[n].x, now[n].y, now[n].z, now[n].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int piece = part * 16 + n * 4 + e;
-          *reinterpret_cast<uint4*>(tile + (piece >> 3) * (kN * 128) + tok * 128 + (((piece & 7) ^ (tok & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(tile + (piece >> 3) * (kN * 128) + (((piece & 7) ^ (tok & 7)) << 4)) =
               make_uint4(mul_bf16x2(kv4_raw<0>(w[e]), f), mul_bf16x2(kv4_raw<1>(w[e]), f), mul_bf16x2(kv4_raw<2>(w[e]), f),
                          mul_bf16x2(kv4_raw<3>(w[e]), f));
         }
       }
-    };
-    bool ok = true;
-    Raw now, next;
-    int page = page_of(0);
-    fetch(now, 0, page);
-    page = page_of(1);
-    for (int i = 0; i < steps && ok; ++i) {
-      if (i + 1 < steps) fetch(next, i + 1, page);
-      page = page_of(i + 2);
-      const int st = i & 1;
-      const uint32_t parity = ((i >> 1) & 1) ^ 1;
-      if (!mbar_wait(&k_empty[st], parity, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
-      store(smem + Cfg::kOffK + st * Cfg::kKBytes, now.k, now.ks);
       fence_proxy_async_smem();
-      mbar_arrive(&k_full[st]);
-      if (!mbar_wait(&v_empty[st], parity, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
-      store(smem + Cfg::kOffV + st * Cfg::kKBytes, now.v, now.vs);
-      fence_proxy_async_smem();
-      mbar_arrive(&v_full[st]);
-      now = next;
+      mbar_arrive(is_v ? &v_full[st] : &k_full[st]);
+#pragma unroll
+      for (int n = 0; n < kWords / 4; ++n) now[n] = next[n];
+      now_s = next_s;
     }
   } else {
     // ---------------------------------------------------------------- products
