@@ -17,8 +17,8 @@
 //
 // Codes become bf16 as in the decode kernel (times 2^-64, exact), in the order 0 4 1 5 2 6 3 7 of
 // each eight channels: Q is stored in the same order, O's columns are put back when written.
-// The maximum that weights refer to moves only when it would grow by more than 2^8, so that O is
-// rescaled in TMEM a few times per row, not once per step.  A weight is the sum of two bf16
+// The maximum that weights refer to moves only when a score passes it by 16 (a factor 2^16), so
+// that O is rescaled in TMEM a few times per row, not once per step.  A weight is the sum of two bf16
 // numbers, to 2^-17: rounded to one it would add as much error to the output as the output's own
 // rounding.  The second product hides behind the exponentials.
 #pragma once
@@ -241,7 +241,8 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     int lo, hi;
     kv4_visible(mask, len - rows + r / q.group, len, lo, hi);
     const float scale = fabsf(mask.scale) * kTwo64;
-    const float s_scale = kCap ? scale / mask.softcap : scale * kLog2e;  // a cap: tanh's argument
+    // with a cap: tanh's argument.  Not zero, so that -inf stays that
+    const float s_scale = fmaxf(kCap ? scale / mask.softcap : scale * kLog2e, 1.2e-38f);
     const float cap2 = kCap ? mask.softcap * kLog2e : 0.f;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     float m = -1e30f, l0 = 0.f, l1 = 0.f;
@@ -270,62 +271,59 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         const uint32_t pages16 = ((there >> (col >> 4)) & 1u ? 0xFFFFu : 0u) | ((there >> ((col >> 4) + 1)) & 1u ? 0xFFFF0000u : 0u);
         return kv4_bits(lo - tb - col, hi - tb - col) & pages16;
       };
-      // the loops over S stay loops: three kinds of warps share the instruction cache
-      float top = -INFINITY, far = 0.f;
-#pragma unroll 1
-      for (int col = 0; col < kN; col += 64) {
-        uint32_t x[2][32];
-        tmem_ld_32x32b_x32(s_at + col, x[0]);
-        tmem_ld_32x32b_x32(s_at + col + 32, x[1]);
-        tc_wait_ld();
-        float t[4] = {top, top, top, top};
-        if (masked) {
-          const uint32_t bits[2] = {seen(col), seen(col + 32)};
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e >> 5][e & 31])));
-            t[e & 3] = fmaxf(t[e & 3], (bits[e >> 5] >> (e & 31)) & 1u ? __uint_as_float(x[e >> 5][e & 31]) : -INFINITY);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e >> 5][e & 31])));
-            t[e & 3] = fmaxf(t[e & 3], __uint_as_float(x[e >> 5][e & 31]));
-          }
-        }
-        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      }
-      top *= s_scale;  // s_scale is not negative; -inf x 0 is not a number, and no maximum
-      const bool near = kCap && __all_sync(0xffffffffu, far * s_scale < 0.4f);  // the series serves (a NaN is not near)
-      if (kCap) top = cap2 * (near ? kv4_tanh_near(top) : kv4_tanh_far(top));
-      const bool grow = top > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float f = grow ? ex2(m - top) : 1.f;
-        if (grow) m = top;
+      // S is read once, 32 columns ahead of the ones worked on; a chunk that would pass 2^16 moves m.
+      // What is rare (and the two halves' loop) stays rolled: three kinds of warps share the
+      // instruction cache.
+      auto raise = [&](float top, bool need, int upto) {  // columns before `upto` hold weights already
+        // m moves by a whole number, so that weights are rescaled exactly
+        const bool fresh = m < -1e29f;
+        const float up = fresh || !need ? 0.f : ceilf(top - m);
+        const float f = fresh && need ? 0.f : __int_as_float(max(127 - static_cast<int>(fminf(up, 127.f)), 0) << 23);
+        m = fresh && need ? top : m + up;
         l0 *= f;
         l1 *= f;
-        if (i > 0) {
-          // one buffer of S: step i's products came after step i - 1's in the pipe.  Two: they may have
-          // come before, but after step i - 2's, so the barrier is in phase i - 1 or just past it
-          if (kSB == 2 && !(ok = wait(&o_done[tile], (i - 1) & 1))) break;
-          tc_fence_after();
+        // one buffer of S: step i's products came after step i - 1's in the pipe.  Two: they may have
+        // come before, but after step i - 2's, so the barrier is in phase i - 1 or just past it
+        if (kSB == 2 && i > 0 && !(ok = wait(&o_done[tile], (i - 1) & 1))) return;
+        tc_fence_after();
 #pragma unroll 1
-          for (int col = 0; col < D; col += 32) {
-            uint32_t x[32];
-            tmem_ld_32x32b_x32(o_at + col, x);
-            tc_wait_ld();
+        for (int col = 0; i > 0 && col < D; col += 32) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32(o_at + col, x);
+          tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-            tmem_st_32x32b_x32(o_at + col, x);
-          }
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+          tmem_st_32x32b_x32(o_at + col, x);
         }
-      }
+        tc_wait_st();
 #pragma unroll 1
-      for (int col = 0; col < kN; col += 32) {
-        uint32_t x[32], p[32];
-        tmem_ld_32x32b_x32(s_at + col, x);
-        tc_wait_ld();
+        for (int col = 0; col < upto; col += 32) {
+          uint32_t x[32];
+          tmem_ld_32x32b_x32(s_at + col, x);
+          tc_wait_ld();
+          const uint32_t f2 = __byte_perm(__float_as_uint(f), 0, 0x3232);  // a power of two: exact as bf16
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = mul_bf16x2(x[e], f2);
+          tmem_st_32x32b_x32(s_at + col, x);
+        }
+      };
+      auto chunk = [&](uint32_t (&x)[32], int col) {
+        uint32_t bits = 0;
+        if (masked) {
+          bits = seen(col);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xFF800000u;
+        }
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, far = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          t[e & 3] = fmaxf(t[e & 3], __uint_as_float(x[e]));
+          if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e])));
+        }
+        float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * s_scale;
         if (kCap) {
+          const bool near = __all_sync(0xffffffffu, far * s_scale < 0.4f);  // the series serves (a NaN is not near)
+          top = top == -INFINITY ? top : cap2 * (near ? kv4_tanh_near(top) : kv4_tanh_far(top));
           if (near) {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
@@ -336,31 +334,42 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(kv4_tanh_far(__uint_as_float(x[e]) * s_scale));
+            for (int e = 0; e < 32; ++e) {
+              x[e] = __float_as_uint(kv4_tanh_far(__uint_as_float(x[e]) * s_scale));
+              if (masked && !((bits >> e) & 1u)) x[e] = 0xFF800000u;
+            }
           }
         }
+        const bool need = top > m + 16.f;
+        if (__any_sync(0xffffffffu, need)) raise(top, need, col);
+        uint32_t pk[32];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
           fma2(y0, y1, kCap ? cap2 : s_scale, -m);
-          x[e] = __float_as_uint(ex2(y0));
-          x[e + 1] = __float_as_uint(ex2(y1));
-        }
-        if (masked) {
-          const uint32_t bits = seen(col);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0u;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float y0 = __uint_as_float(x[2 * e]), y1 = __uint_as_float(x[2 * e + 1]);
+          y0 = ex2(y0);
+          y1 = ex2(y1);
           add2(l0, l1, y0, y1);
-          p[e] = pack_bf16x2(y0, y1);
-          sub2(y0, y1, __uint_as_float(p[e] << 16), __uint_as_float(p[e] & 0xFFFF0000u));
-          p[16 + e] = pack_bf16x2(y0, y1);
+          const uint32_t p = pack_bf16x2(y0, y1);
+          sub2(y0, y1, __uint_as_float(p << 16), __uint_as_float(p & 0xFFFF0000u));
+          // first terms to the chunk's first 16 columns, second terms to the others
+          pk[e >> 1] = p;
+          pk[16 + (e >> 1)] = pack_bf16x2(y0, y1);
         }
-        tmem_st_32x32b_x32(s_at + col, p);  // over the columns just read
+        tmem_st_32x32b_x32(s_at + col, pk);  // over the columns just read
+      };
+      uint32_t xa[32], xb[32];
+      tmem_ld_32x32b_x32(s_at, xa);
+#pragma unroll 1
+      for (int col = 0; col < kN && ok; col += 64) {
+        tc_wait_ld();
+        tmem_ld_32x32b_x32(s_at + col + 32, xb);
+        chunk(xa, col);
+        tc_wait_ld();
+        if (col + 64 < kN) tmem_ld_32x32b_x32(s_at + col + 64, xa);
+        chunk(xb, col + 32);
       }
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[tile * kSB + buf]);
