@@ -17,8 +17,8 @@
 //
 // Codes become bf16 as in the decode kernel (times 2^-64, exact), in the order 0 4 1 5 2 6 3 7 of
 // each eight channels: Q is stored in the same order, O's columns are put back when written.
-// The maximum that weights refer to moves only when a score passes it by 16 (a factor 2^16), so
-// that O is rescaled in TMEM a few times per row, not once per step.  A weight is the sum of two bf16
+// What weights refer to, m, is a score of the row and moves only when weights become large (a
+// chunk's sum above 2^20), so that O is rescaled in TMEM a few times per row, not once per step.  A weight is the sum of two bf16
 // numbers, to 2^-17: rounded to one it would add as much error to the output as the output's own
 // rounding.  The second product hides behind the exponentials.
 #pragma once
@@ -271,7 +271,8 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         const uint32_t pages16 = ((there >> (col >> 4)) & 1u ? 0xFFFFu : 0u) | ((there >> ((col >> 4) + 1)) & 1u ? 0xFFFF0000u : 0u);
         return kv4_bits(lo - tb - col, hi - tb - col) & pages16;
       };
-      // S is read once, 32 columns ahead of the ones worked on; a chunk that would pass 2^16 moves m.
+      // S is read once, 32 columns ahead of the ones worked on; a chunk whose weights sum to more than
+      // 2^20 moves m and is done again.
       // What is rare (and the two halves' loop) stays rolled: three kinds of warps share the
       // instruction cache.
       auto raise = [&](float top, bool need, int upto) {  // columns before `upto` hold weights already
@@ -314,16 +315,11 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xFF800000u;
         }
-        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, far = 0.f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          t[e & 3] = fmaxf(t[e & 3], __uint_as_float(x[e]));
-          if (kCap) far = fmaxf(far, fabsf(__uint_as_float(x[e])));
-        }
-        float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * s_scale;
         if (kCap) {
+          float far = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) far = fmaxf(far, fabsf(__uint_as_float(x[e])));
           const bool near = __all_sync(0xffffffffu, far * s_scale < 0.4f);  // the series serves (a NaN is not near)
-          top = top == -INFINITY ? top : cap2 * (near ? kv4_tanh_near(top) : kv4_tanh_far(top));
           if (near) {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
@@ -340,22 +336,35 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
             }
           }
         }
-        const bool need = top > m + 16.f;
-        if (__any_sync(0xffffffffu, need)) raise(top, need, col);
+        const float k = kCap ? cap2 : s_scale;
         uint32_t pk[32];
+        float c0, c1;
+        // weights of the chunk, first terms to its first 16 columns, second terms to the others
+        auto weigh = [&]() {
+          c0 = c1 = 0.f;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
-          fma2(y0, y1, kCap ? cap2 : s_scale, -m);
-          y0 = ex2(y0);
-          y1 = ex2(y1);
-          add2(l0, l1, y0, y1);
-          const uint32_t p = pack_bf16x2(y0, y1);
-          sub2(y0, y1, __uint_as_float(p << 16), __uint_as_float(p & 0xFFFF0000u));
-          // first terms to the chunk's first 16 columns, second terms to the others
-          pk[e >> 1] = p;
-          pk[16 + (e >> 1)] = pack_bf16x2(y0, y1);
+          for (int e = 0; e < 32; e += 2) {
+            float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
+            fma2(y0, y1, k, -m);
+            y0 = ex2(y0);
+            y1 = ex2(y1);
+            add2(c0, c1, y0, y1);
+            const uint32_t p = pack_bf16x2(y0, y1);
+            sub2(y0, y1, __uint_as_float(p << 16), __uint_as_float(p & 0xFFFF0000u));
+            pk[e >> 1] = p;
+            pk[16 + (e >> 1)] = pack_bf16x2(y0, y1);
+          }
+        };
+        weigh();
+        // the sum tells, without a maximum for each element, that a weight has become too large
+        if (__any_sync(0xffffffffu, c0 + c1 > 1048576.f)) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+          raise(top * k, top * k > m, col);
+          weigh();
         }
+        add2(l0, l1, c0, c1);
         tmem_st_32x32b_x32(s_at + col, pk);  // over the columns just read
       };
       uint32_t xa[32], xb[32];
