@@ -163,7 +163,9 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   float* partial = reinterpret_cast<float*>(desc + grid);
   int rc = launch(b2g_kv4_decode_kernel<D, NT>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
   if (rc) return rc;
-  return launch(b2g_kv4_join_kernel<D, NT>, dim3(grid, 2 * NT), 512, 0, f.st, f.bt, q, o, partial, desc);
+  // blocks of four rows for items in many parts took 2 us more wherever most have nothing to join
+  constexpr int kWide = NT == 1 ? 8 : 16;
+  return launch(b2g_kv4_join_kernel<D, NT, kWide>, dim3(grid, 8 * NT / kWide), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
 template <int D, bool kCap>

@@ -52,6 +52,7 @@ struct Kv4Out {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kTwo64 = 18446744073709551616.f;
+constexpr float kNoMax = -1e30f;  // the maximum of nothing: finite, so that differences are numbers
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -281,7 +282,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4Out& out, long long row, int
   const float f = l == 0.f ? 0.f : kTwo64 / l;
   const int ch = 32 * (pair >> 4) + 4 * (pair & 7) + 2 * ((pair >> 3) & 1);
   *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(v.x * f, v.y * f);
-  if (pair == 0) out.lse[row * heads + head] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) * kLn2 + logf(l);
+  if (pair == 0) out.lse[row * heads + head] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 template <int D, int NT>
@@ -366,17 +367,17 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     if (lane == 0) s_there[stage] = there;
     const uint32_t dst = smem_u32(ring + stage * Cfg::kStage);
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int n = i * 32 + lane;
-      const int token = n / kChunks, ch = n % kChunks;
-      const int grp = token >> 4, tau = token & 15;
-      // ldmatrix reads a piece of eight tokens at once: those eight lie in distinct banks
-      const int at_ch = ch ^ (D == 256 ? tau & 7 : D == 128 ? (tau >> 1) & 3 : (tau >> 2) & 1);
-      const long long src = ((grp ? at[1] : at[0]) + tau) * (D / 2) + ch * 16;
+    for (int grp = 0; grp < 2; ++grp) {  // 16 tokens, contiguous in their page
+      const long long from = at[grp] * (D / 2) + lane * 16;
       const bool ok = (there >> grp) & 1;
-      const uint32_t to = dst + token * (D / 2) + at_ch * 16;
-      cp_async16(to, c.k + src, ok);
-      cp_async16(to + Cfg::kHalf, c.v + src, ok);
+#pragma unroll
+      for (int j = 0; j < kChunks / 2; ++j) {
+        const int tau = (j * 32 + lane) / kChunks, ch = (j * 32 + lane) % kChunks;
+        // ldmatrix reads a piece of eight tokens at once: those eight lie in distinct banks
+        const uint32_t to = dst + (grp * 16 + tau) * (D / 2) + ((ch ^ (D == 256 ? tau & 7 : D == 128 ? (tau >> 1) & 3 : (tau >> 2) & 1)) * 16);
+        cp_async16(to, c.k + from + j * 512, ok);
+        cp_async16(to + Cfg::kHalf, c.v + from + j * 512, ok);
+      }
     }
     if (lane < 4 * kChunks) {
       const bool is_v = lane >= 2 * kChunks;
@@ -424,7 +425,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     float rs[NT][2], m[NT][2], l[NT][2], o[kMT][NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = kNoMax;
       l[nt][0] = l[nt][1] = 0.f;
       rs[nt][0] = s_rs[nt * 8 + 2 * t];
       rs[nt][1] = s_rs[nt * 8 + 2 * t + 1];
@@ -554,7 +555,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
           if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float f = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - top[e]);
+              const float f = ex2(m[nt][e] - top[e]);
               m[nt][e] = top[e];
               l[nt][e] *= f;
 #pragma unroll
@@ -572,9 +573,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
           uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-            const float p0 = ex2(s[tile][nt][0] - m0), p1 = ex2(s[tile][nt][1] - m1);
-            const float p2 = ex2(s[tile][nt][2] - m0), p3 = ex2(s[tile][nt][3] - m1);
+            const float p0 = ex2(s[tile][nt][0] - m[nt][0]), p1 = ex2(s[tile][nt][1] - m[nt][1]);
+            const float p2 = ex2(s[tile][nt][2] - m[nt][0]), p3 = ex2(s[tile][nt][3] - m[nt][1]);
             l[nt][0] += p0 + p2;
             l[nt][1] += p1 + p3;
             // a weight is the sum of two bf16 numbers, to 2^-17: rounded to one alone it would add as
@@ -650,8 +650,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float mw = s_m[w * kRows + r];
-          // a row all of whose scores are NaN has no maximum, but a sum that is NaN
-          const float f = mw == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : ex2(mw - top);
+          const float f = ex2(mw - top);
           sum += f * s_l[w * kRows + r];
           const float2 x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem + (w * kStages + used) * Cfg::kStage) +
                                                             (r - nt * 8) * Cfg::kMergeStride + 2 * pair);
@@ -684,12 +683,12 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   griddep_launch_dependents();
 }
 
-// Joins the parts of an item that was cut: block (i, y) has rows 4 y .. 4 y + 3 of the item that
-// decode CTA i began.  512 threads: four warps share a row's parts, eight in flight each.
-template <int D, int NT>
+// Joins the parts of an item that was cut: block (i, y) has kRB rows from kRB y on of the item that
+// decode CTA i began.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
+template <int D, int NT, int kRB>
 __global__ void __launch_bounds__(512)
 b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial, const int4* __restrict__ desc) {
-  constexpr int kRows = 8 * NT, kE = D / 32, kShare = 4;
+  constexpr int kRows = 8 * NT, kE = D / 32, kShare = 16 / kRB;
   __shared__ float s_o[16][D];
   __shared__ float s_m[16], s_l[16];
   griddep_wait();
@@ -701,10 +700,8 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
   const int blocks = (group_rows + kRows - 1) / kRows;
   const int h = d.z / blocks, r0 = (d.z - h * blocks) * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = warp % kShare, r = blockIdx.y * 4 + warp / kShare;
-  float top = -INFINITY, sum = 0.f, o[kE] = {};
-  // a part without a maximum weighs nothing, unless none has one: then sums that are NaN come through
-  auto weight = [](float m, float t) { return m == -INFINITY ? (t == -INFINITY ? 1.f : 0.f) : ex2(m - t); };
+  const int share = warp % kShare, r = blockIdx.y * kRB + warp / kShare;
+  float top = kNoMax, sum = 0.f, o[kE] = {};
   if (r0 + r < group_rows) {
 #pragma unroll 1
     for (int i0 = share; i0 < d.x; i0 += 8 * kShare) {
@@ -712,7 +709,7 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int i = i0 + j * kShare;
-        mm[j] = -INFINITY;
+        mm[j] = kNoMax;
         ll[j] = 0.f;
 #pragma unroll
         for (int e = 0; e < kE; ++e) x[j][e] = 0.f;
@@ -731,13 +728,13 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
       float t = top;
 #pragma unroll
       for (int j = 0; j < 8; ++j) t = fmaxf(t, mm[j]);
-      const float f = weight(top, t);
+      const float f = ex2(top - t);
       sum *= f;
 #pragma unroll
       for (int e = 0; e < kE; ++e) o[e] *= f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float g = weight(mm[j], t);
+        const float g = ex2(mm[j] - t);
         sum += g * ll[j];
 #pragma unroll
         for (int e = 0; e < kE; ++e) o[e] += g * x[j][e];
@@ -753,13 +750,13 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
   float t = top;
 #pragma unroll
   for (int w = 1; w < kShare; ++w) t = fmaxf(t, s_m[warp + w]);
-  const float f = weight(top, t);
+  const float f = ex2(top - t);
   sum *= f;
 #pragma unroll
   for (int e = 0; e < kE; ++e) o[e] *= f;
 #pragma unroll
   for (int w = 1; w < kShare; ++w) {
-    const float g = weight(s_m[warp + w], t);
+    const float g = ex2(s_m[warp + w] - t);
     sum += g * s_l[warp + w];
 #pragma unroll
     for (int e = 0; e < kE; ++e) o[e] += g * s_o[warp + w][(e & ~1) * 32 + 2 * lane + (e & 1)];

@@ -9,18 +9,18 @@
 // Warps: one softmax warpgroup per query tile, four warps that turn codes into bf16 tiles, one
 // that issues the products.
 //
-// What bounds it: for D = 128 the 2 x 128 x 128 exponentials of a step take 2048 clocks of the
-// SM's 16 a clock; the products take 1536, decoding 32768 codes ~700 issue slots a scheduler.
-// Hence two query tiles: while one's S is being exponentiated the other's products run, and what
-// a step decodes serves 256 rows.  D = 256 leaves TMEM for one query tile, whose S has two
-// buffers instead.
+// What bounds it: for D = 128 the products of a step take 3072 clocks at 4096 multiplications a
+// clock, its 2 x 128 x 128 exponentials 2048 at 16 a clock, decoding 32768 codes ~700 issue slots a
+// scheduler.  Hence two query tiles: while one's S is being exponentiated the other's products
+// run, and what a step decodes serves 256 rows.  D = 256 leaves TMEM for one query tile, whose S
+// has two buffers instead.
 //
 // Codes become bf16 as in the decode kernel (times 2^-64, exact), in the order 0 4 1 5 2 6 3 7 of
 // each eight channels: Q is stored in the same order, O's columns are put back when written.
 // What weights refer to, m, is a score of the row and moves only when weights become large (a
-// chunk's sum above 2^20), so that O is rescaled in TMEM a few times per row, not once per step.  A weight is the sum of two bf16
-// numbers, to 2^-17: rounded to one it would add as much error to the output as the output's own
-// rounding.  The second product hides behind the exponentials.
+// chunk's sum above 2^20), so that O is rescaled in TMEM a few times per row, not once per step.
+// A weight is the sum of two bf16 numbers, to 2^-17: rounded to one it would add as much error to
+// the output as the output's own rounding.  That is a third of the products' time.
 #pragma once
 
 #include "b2g_kv4_decode.cuh"
@@ -413,8 +413,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     // ---------------------------------------------------------------- codes to bf16 tiles
     // K of a step, then V, by the same code: halves are fetched one ahead, page numbers a step ahead
     constexpr int kWords = D == 64 ? 8 : 16;  // a thread's words of a half
-    constexpr int kPer = D == 256 ? 2 : 1;    // threads to a token
-    const int dt = threadIdx.x - kDecodeWarp * 32, tok = dt / kPer, part = dt % kPer;
+    const int dt = threadIdx.x - kDecodeWarp * 32, tok = dt % kN, part = dt / kN;  // a warp's lanes: consecutive tokens
     auto page_of = [&](int i) {
       const int token = (j0 + i) * kN + tok;
       return i < steps && token < len ? __ldg(pages + (token >> c.page_log2)) : -2;
