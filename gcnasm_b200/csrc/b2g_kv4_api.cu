@@ -149,23 +149,23 @@ int resident(K kernel, int block, size_t smem, int most, int dev, std::atomic<in
   return n;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kTwin>
 int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, void* workspace) {
-  using Cfg = DecodeCfg<D, NT>;
+  using Cfg = DecodeCfg<D, NT, kTwin>;
   static std::atomic<int> few[64], many[64];
   // room for the prefix sums of 512 sequences, or of as many as there can be
   const bool is_few = f.bt.seqs <= 512;
   const size_t smem = ((Cfg::kFixed + 15) & ~15) + ((is_few ? 512 : 8192) + 1) * sizeof(long long);
-  const int n = resident(b2g_kv4_decode_kernel<D, NT>, 128, smem, decode_ctas(NT), f.dev, is_few ? few : many);
+  const int n = resident(b2g_kv4_decode_kernel<D, NT, kTwin>, 128, smem, decode_ctas(NT), f.dev, is_few ? few : many);
   if (n < 1) return host_fail(B2G_ERR_CUDA, "the decode kernel does not fit on the device");
   const int grid = n * f.sms;
   int4* desc = static_cast<int4*>(workspace);
   float* partial = reinterpret_cast<float*>(desc + grid);
-  int rc = launch(b2g_kv4_decode_kernel<D, NT>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
+  int rc = launch(b2g_kv4_decode_kernel<D, NT, kTwin>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
   if (rc) return rc;
   // blocks of four rows for items in many parts took 2 us more wherever most have nothing to join
-  constexpr int kWide = NT == 1 ? 8 : 16;
-  return launch(b2g_kv4_join_kernel<D, NT, kWide>, dim3(grid, 8 * NT / kWide), 512, 0, f.st, f.bt, q, o, partial, desc);
+  constexpr int kRB = std::min(Cfg::kRows, 16);
+  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, kRB>, dim3(grid, Cfg::kRows / kRB), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
 template <int D, bool kCap>
@@ -264,9 +264,10 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (rows >= kPromptRows) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, rows) : prompt<D, false>(f, m, qs, o, rows);
-    else if (rows <= 8) rc = decode<D, 1>(f, m, qs, o, workspace);
-    else if (rows <= 16 || D == 256) rc = decode<D, 2>(f, m, qs, o, workspace);
-    else if constexpr (D < 256) rc = decode<D, 4>(f, m, qs, o, workspace);
+    else if (rows <= 4) rc = decode<D, 1, true>(f, m, qs, o, workspace);
+    else if (rows <= 8) rc = decode<D, 1, false>(f, m, qs, o, workspace);
+    else if (rows <= 16 || D == 256) rc = decode<D, 2, false>(f, m, qs, o, workspace);
+    else if constexpr (D < 256) rc = decode<D, 4, false>(f, m, qs, o, workspace);
   });
   return rc;
 }

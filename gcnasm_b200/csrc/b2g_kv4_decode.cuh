@@ -100,6 +100,14 @@ __device__ __forceinline__ void mma_bf16_16816(float (&c)[4], uint32_t a0, uint3
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same into fresh sums
+__device__ __forceinline__ void mma_f16_16816_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                  uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -216,21 +224,21 @@ __device__ __forceinline__ int kv4_seq_of_unit(const long long* pre, int seqs, l
   return lo;
 }
 
-// 8 NT query rows of a kv head, from row n0 of its group_rows, as B fragments in f16: each row
+// 8 NT query rows (kTwin: four, twice) of a kv head, from row n0 of its group_rows, as B fragments in f16: each row
 // times a power of two that puts its largest element in [2^14, 2^15), whose inverse times `scale`
 // goes to s_rs.  s_top: zeros, 8 NT, and the caller clears it behind the barrier that follows.
-template <int D, int NT, int kThreads>
+template <int D, int NT, bool kTwin>
 __device__ __forceinline__ void kv4_stage_q(const Kv4Queries& q, int first, int h, int n0, int group_rows, float scale, uint2* s_q,
                                             int* s_top, float* s_rs) {
   auto q_of = [&](int i, int& r) {
     const int ln = i & 31, nt = (i >> 5) % NT, blk = (i >> 5) / NT;
     r = nt * 8 + (ln >> 2);
-    const int n = n0 + r;
+    const int n = n0 + (kTwin ? r & 3 : r);
     if (n >= group_rows) return make_uint4(0, 0, 0, 0);
     return __ldg(reinterpret_cast<const uint4*>(q.q + (first + n / q.group) * q.q_row + (h * q.group + n % q.group) * q.q_head +
                                                 32 * blk + 8 * (ln & 3)));
   };
-  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += kThreads) {
+  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += 128) {
     int r;
     const uint4 x = q_of(i, r);
     uint32_t top = 0;  // magnitudes as integers
@@ -238,7 +246,7 @@ __device__ __forceinline__ void kv4_stage_q(const Kv4Queries& q, int first, int 
     atomicMax(&s_top[r], static_cast<int>(top));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += kThreads) {
+  for (int i = threadIdx.x; i < (D / 32) * NT * 32; i += 128) {
     int r;
     const uint4 x = q_of(i, r);
     const int ex = min(max(s_top[r] >> 23, 27), 254);  // the largest element is below 2^(ex - 126)
@@ -252,9 +260,13 @@ __device__ __forceinline__ void kv4_stage_q(const Kv4Queries& q, int first, int 
   __syncthreads();
 }
 
-template <int D, int NT>
+// kTwin: up to four rows, each twice in a tile of eight -- the second time with the weights'
+// second terms, which then take no product of their own (decode_batch: 8 us of 97).
+template <int D, int NT, bool kTwin>
 struct DecodeCfg {
-  static constexpr int kRows = 8 * NT;
+  static_assert(!kTwin || NT == 1, "one tile of eight");
+  static constexpr int kPad = 8 * NT;                 // rows in tiles
+  static constexpr int kRows = kTwin ? 4 : kPad;      // query rows
   static constexpr int kChunks = D / 32;              // 16-byte pieces of a token's K (or V), and its scales
   static constexpr int kHalf = 32 * (D / 2);          // bytes of 32 tokens' K
   static constexpr int kStage = 2 * kHalf + 64 * kChunks;
@@ -265,7 +277,7 @@ struct DecodeCfg {
   static_assert(8 * kMergeStride * 4 <= kStage, "a warp's eight rows of O lie in the stage it has just used");
   static constexpr int kQ = (D / 16) * NT * 256;      // Q as B fragments
   static constexpr int kScales = 4 * 32 * kChunks;    // scales of a warp's 32 tokens as bf16
-  static constexpr int kFixed = 4 * (kStages * kStage + kScales + kStages * 4) + kQ + (2 * 4 + 2) * kRows * 4;
+  static constexpr int kFixed = 4 * (kStages * kStage + kScales + kStages * 4) + kQ + (2 * 4 + 2) * kPad * 4;
 };
 
 // Position of an item's units among all, walked unit by unit.
@@ -285,12 +297,12 @@ __device__ __forceinline__ void kv4_finish(const Kv4Out& out, long long row, int
   if (pair == 0) out.lse[row * heads + head] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kTwin>
 __global__ void __launch_bounds__(128, NT == 1 && D < 256 ? 3 : 2)
 b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, float* __restrict__ partial,
                       int4* __restrict__ desc, int* status) {
-  using Cfg = DecodeCfg<D, NT>;
-  constexpr int kRows = Cfg::kRows, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
+  using Cfg = DecodeCfg<D, NT, kTwin>;
+  constexpr int kRows = Cfg::kRows, kPad = Cfg::kPad, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
   constexpr int kMT = D / 16;  // 16-channel tiles of O
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -299,11 +311,11 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   uint8_t* s_scales = reinterpret_cast<uint8_t*>(s_q) + Cfg::kQ + warp * Cfg::kScales;
   uint8_t* s_ks = s_scales;                      // K's: [32][kChunks] bf16
   uint16_t* s_vs = reinterpret_cast<uint16_t*>(s_scales + 64 * kChunks);  // V's: [kChunks][32] bf16
-  float* s_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + Cfg::kQ + 4 * Cfg::kScales);  // [4][kRows]
-  float* s_l = s_m + 4 * kRows;
-  float* s_rs = s_l + 4 * kRows;                 // what turns a row's sums into scores
-  int* s_top = reinterpret_cast<int*>(s_rs + kRows);
-  int* s_there = s_top + kRows + warp * kStages;  // per stage: which groups of 16 are there
+  float* s_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(s_q) + Cfg::kQ + 4 * Cfg::kScales);  // [4][kPad]
+  float* s_l = s_m + 4 * kPad;
+  float* s_rs = s_l + 4 * kPad;                  // what turns a row's sums into scores
+  int* s_top = reinterpret_cast<int*>(s_rs + kPad);
+  int* s_there = s_top + kPad + warp * kStages;  // per stage: which groups of 16 are there
   long long* s_pre = reinterpret_cast<long long*>(smem + ((Cfg::kFixed + 15) & ~15));  // [seqs + 1] units before
   __shared__ long long s_scan[4];
 
@@ -409,14 +421,14 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   const int lm_tok = (lane & 7) + (lane & 8), lm_ch = lane >> 4;
   const uint32_t lm_row = lm_tok * (D / 2);
   const int lm_swz = D == 256 ? lm_tok & 7 : D == 128 ? (lm_tok >> 1) & 3 : (lm_tok >> 2) & 1;
-  if (tid < kRows) s_top[tid] = 0;
+  if (tid < kPad) s_top[tid] = 0;
   __syncthreads();
   int stage = 0;
   long long u = u0;
   while (u < u1) {
     const int group_rows = cw.s.rows * q.group;
-    kv4_stage_q<D, NT, 128>(q, cw.s.first, cw.h, cw.rb * kRows, group_rows, s_scale, s_q, s_top, s_rs);
-    if (tid < kRows) s_top[tid] = 0;  // for the next item, behind this one's barriers
+    kv4_stage_q<D, NT, kTwin>(q, cw.s.first, cw.h, cw.rb * kRows, group_rows, s_scale, s_q, s_top, s_rs);
+    if (tid < kPad) s_top[tid] = 0;  // for the next item, behind this one's barriers
     uint2 qr[NT == 1 ? D / 16 : 1];
     if (NT == 1) {
 #pragma unroll
@@ -502,8 +514,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
               for (int nt = 0; nt < NT; ++nt) {
                 const uint2 b0 = NT == 1 ? qr[2 * blk] : s_q[(2 * blk * NT + nt) * 32 + lane];
                 const uint2 b1 = NT == 1 ? qr[2 * blk + 1] : s_q[((2 * blk + 1) * NT + nt) * 32 + lane];
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16_16816(x, a[0], b[0], a[1], b[1], b0.x, b0.y);
+                float x[4];
+                mma_f16_16816_new(x, a[0], b[0], a[1], b[1], b0.x, b0.y);
                 mma_f16_16816(x, a[2], b[2], a[3], b[3], b1.x, b1.y);
                 if (blk == 0) {
                   s[tile][nt][0] = x[0] * g0, s[tile][nt][1] = x[1] * g0;
@@ -533,7 +545,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               int lo, hi;
-              kv4_visible(mask, ps.len - ps.rows + (r0 + nt * 8 + 2 * t + e) / q.group, ps.len, lo, hi);
+              kv4_visible(mask, ps.len - ps.rows + (r0 + nt * 8 + ((2 * t + e) & (kTwin ? 3 : 7))) / q.group, ps.len, lo, hi);
 #pragma unroll
               for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
@@ -580,10 +592,14 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
             // a weight is the sum of two bf16 numbers, to 2^-17: rounded to one alone it would add as
             // much error to the output as the output's own rounding
             const uint32_t h0 = pack_bf16x2(p0, p1), h1 = pack_bf16x2(p2, p3);
-            hi[nt][0] = movmatrix_trans(h0);
-            hi[nt][1] = movmatrix_trans(h1);
-            lo[nt][0] = movmatrix_trans(pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xFFFF0000u)));
-            lo[nt][1] = movmatrix_trans(pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xFFFF0000u)));
+            const uint32_t l0 = pack_bf16x2(p0 - __uint_as_float(h0 << 16), p1 - __uint_as_float(h0 & 0xFFFF0000u));
+            const uint32_t l1 = pack_bf16x2(p2 - __uint_as_float(h1 << 16), p3 - __uint_as_float(h1 & 0xFFFF0000u));
+            hi[nt][0] = movmatrix_trans(kTwin && t >= 2 ? l0 : h0);
+            hi[nt][1] = movmatrix_trans(kTwin && t >= 2 ? l1 : h1);
+            if (!kTwin) {
+              lo[nt][0] = movmatrix_trans(l0);
+              lo[nt][1] = movmatrix_trans(l1);
+            }
           }
 #pragma unroll
           for (int pair = 0; pair < kChunks / 2; ++pair) {
@@ -603,9 +619,9 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma_bf16_16816(o[2 * blk][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
-                mma_bf16_16816(o[2 * blk][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
+                if (!kTwin) mma_bf16_16816(o[2 * blk][nt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
                 mma_bf16_16816(o[2 * blk + 1][nt], c0, c1, c2, c3, hi[nt][0], hi[nt][1]);
-                mma_bf16_16816(o[2 * blk + 1][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
+                if (!kTwin) mma_bf16_16816(o[2 * blk + 1][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
               }
             }
           }
@@ -631,29 +647,34 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 #pragma unroll
         for (int sh = 4; sh <= 16; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
         if (g == 0) {
-          s_m[warp * kRows + nt * 8 + 2 * t + e] = m[nt][e];
-          s_l[warp * kRows + nt * 8 + 2 * t + e] = sum;
+          s_m[warp * kPad + nt * 8 + 2 * t + e] = m[nt][e];
+          s_l[warp * kPad + nt * 8 + 2 * t + e] = sum;
         }
 #pragma unroll
         for (int i = 0; i < kMT; ++i)
           *reinterpret_cast<float2*>(mine + (2 * t + e) * Cfg::kMergeStride + i * 16 + 2 * g) = make_float2(o[i][nt][e], o[i][nt][2 + e]);
       }
       __syncthreads();
-      for (int i = tid; i < 8 * (D / 2); i += 128) {
+      for (int i = tid; i < (kTwin ? 4 : 8) * (D / 2); i += 128) {
         const int r = nt * 8 + i / (D / 2), pair = i % (D / 2);
         if (r0 + r > r1) break;
         float top = s_m[r];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * kRows + r]);
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w * kPad + r]);
         float sum = 0.f;
         float2 v = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float mw = s_m[w * kRows + r];
+          const float mw = s_m[w * kPad + r];
           const float f = ex2(mw - top);
-          sum += f * s_l[w * kRows + r];
-          const float2 x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem + (w * kStages + used) * Cfg::kStage) +
-                                                            (r - nt * 8) * Cfg::kMergeStride + 2 * pair);
+          sum += f * s_l[w * kPad + r];
+          const float* from = reinterpret_cast<const float*>(smem + (w * kStages + used) * Cfg::kStage) + (r - nt * 8) * Cfg::kMergeStride + 2 * pair;
+          float2 x = *reinterpret_cast<const float2*>(from);
+          if (kTwin) {
+            const float2 y = *reinterpret_cast<const float2*>(from + 4 * Cfg::kMergeStride);
+            x.x += y.x;
+            x.y += y.y;
+          }
           v.x += f * x.x;
           v.y += f * x.y;
         }
@@ -685,10 +706,10 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 
 // Joins the parts of an item that was cut: block (i, y) has kRB rows from kRB y on of the item that
 // decode CTA i began.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
-template <int D, int NT, int kRB>
+template <int D, int kRows, int kRB>
 __global__ void __launch_bounds__(512)
 b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial, const int4* __restrict__ desc) {
-  constexpr int kRows = 8 * NT, kE = D / 32, kShare = 16 / kRB;
+  constexpr int kE = D / 32, kShare = 16 / kRB;
   __shared__ float s_o[16][D];
   __shared__ float s_m[16], s_l[16];
   griddep_wait();
