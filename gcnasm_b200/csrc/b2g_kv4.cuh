@@ -82,87 +82,82 @@ __device__ __forceinline__ int kv4_scale_byte(float amax) {
   return min(max(byte, kKv4ScaleMin), kKv4ScaleMax);
 }
 
-constexpr int kRowsDeep = 2;
-
 // Tokens of a row-wise kernel: thread `in` of a row's per_row, over all rows.  A block of 256
-// threads has 256 / per_row rows at a time, or a row in several goes, and takes kRowsDeep of such
-// steps together so that as many walks from row to page are under way; all its threads take the
-// same number of steps, so that lanes can exchange.  f(rows, in, live), a row each of the steps.
+// threads has 256 / per_row rows at a time, or a row in several goes; all its threads take the
+// same number of steps, so that lanes can exchange.  f(row, in, live)
 template <typename F>
 __device__ __forceinline__ void kv4_for_rows(int rows, int per_row, F&& f) {
   const int at_once = max(1, 256 / per_row);
   const int sub = per_row < 256 ? static_cast<int>(threadIdx.x) / per_row : 0;
   const int in0 = static_cast<int>(threadIdx.x) - sub * per_row;
-  const long long step = static_cast<long long>(gridDim.x) * at_once;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * at_once; row0 < rows; row0 += kRowsDeep * step) {
-    for (int in = in0; in - in0 < per_row; in += 256) {
-      int row[kRowsDeep];
-      bool live[kRowsDeep];
-#pragma unroll
-      for (int i = 0; i < kRowsDeep; ++i) {
-        live[i] = sub < at_once && row0 + i * step + sub < rows && in < per_row;
-        row[i] = live[i] ? static_cast<int>(row0 + i * step) + sub : 0;
-      }
-      f(row, in < per_row ? in : 0, live);
-    }
+  for (long long row0 = static_cast<long long>(blockIdx.x) * at_once; row0 < rows; row0 += static_cast<long long>(gridDim.x) * at_once) {
+    const int row = static_cast<int>(row0) + sub;
+    const bool live = sub < at_once && row0 + sub < rows;
+    for (int in = in0; in - in0 < per_row; in += 256) f(live ? row : 0, live && in < per_row ? in : 0, live && in < per_row);
   }
 }
 
+// Eight values as E2M1 codes, the first in the low bits: nearest, a tie to the even code,
+// saturating at 6; a NaN becomes 6.
+__device__ __forceinline__ uint32_t e2m1x8(const float* x) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
-// append: one thread per 8 channels of a token's K and V, four threads per scale block, so a
-// warp reads 1 KB (bf16) and writes 256 bytes, and the walk from row to page is paid once for
-// both.  Bound by bytes: the input is 4 (bf16) or 8 (fp32) of 5.06 or 9.06 moved per value pair.
+// append: one thread per 16 channels of a token's K and V, two threads per scale block: the
+// walk from row to page, which took half of the instructions with 8 channels of one of them, is paid
+// once for 32 values.  Bound by bytes: the input is 4 (bf16) or 8 (fp32) of 5.06 or 9.06 moved per value pair.
 // ---------------------------------------------------------------------------
 template <typename In, int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_append_kernel(Kv4Cache c, Kv4Batch bt, const In* __restrict__ k, const In* __restrict__ v, long long k_row,
                       long long k_head, long long v_row, long long v_head, float* __restrict__ weights,
                       int* status) {
-  constexpr int kPer = D / 8;  // threads of one head
+  constexpr int kPer = D / 16;  // threads of one head
   griddep_wait();
-  kv4_for_rows(bt.rows, c.heads * kPer, [&](const int (&row)[kRowsDeep], int in, const bool (&live)[kRowsDeep]) {
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
     const int head = in / kPer, g = in % kPer;
-    float x[kRowsDeep][2][8] = {};
-#pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n)
-      if (live[n]) {
-        load8_f32(k + row[n] * k_row + head * k_head + g * 8, x[n][0]);
-        load8_f32(v + row[n] * v_row + head * v_head + g * 8, x[n][1]);
-      }
-    long long at[kRowsDeep];
-#pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n) {
-      at[n] = -1;
-      if (live[n]) {
-        const int b = kv4_seq_of_row(bt, row[n]);
-        int first, end;
-        kv4_rows(bt, b, first, end);
-        const int len = kv4_len(bt, b, c.page_log2);
-        const int token = __ldg(bt.lens + b) - (end - row[n]);
-        if (row[n] >= first && row[n] < end && token >= 0 && token < len)
-          at[n] = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, token, status);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n) {
+    float x[2][2][8] = {};
+    if (live) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float amax = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[n][i][j]));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        if (at[n] < 0) continue;
-        const int byte = kv4_scale_byte(amax);
-        const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
-        uint32_t pk = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pk |= f32_to_e2m1(x[n][i][j] * inv) << (4 * j);
-        *reinterpret_cast<uint32_t*>((i ? c.v : c.k) + at[n] * (D / 2) + g * 4) = pk;
-        if ((g & 3) == 0) (i ? c.vs : c.ks)[at[n] * (D / 32) + (g >> 2)] = static_cast<uint8_t>(byte);
+        const In* from = (i ? v + row * v_row + head * v_head : k + row * k_row + head * k_head) + g * 16;
+        load8_f32(from, x[i][0]);
+        load8_f32(from + 8, x[i][1]);
       }
-      if (at[n] >= 0 && weights && g == 0) weights[at[n]] = 0.f;
     }
+    long long at = -1;
+    if (live) {
+      const int b = kv4_seq_of_row(bt, row);
+      int first, end;
+      kv4_rows(bt, b, first, end);
+      const int len = kv4_len(bt, b, c.page_log2);
+      const int token = __ldg(bt.lens + b) - (end - row);
+      if (row >= first && row < end && token >= 0 && token < len)
+        at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, token, status);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(x[i][j >> 3][j & 7]));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      if (at < 0) continue;
+      const int byte = kv4_scale_byte(amax);
+      const float inv = __int_as_float((254 - byte) << 23);  // 2^(127 - byte), exact
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[i][j >> 3][j & 7] *= inv;
+      *reinterpret_cast<uint2*>((i ? c.v : c.k) + at * (D / 2) + g * 8) = make_uint2(e2m1x8(x[i][0]), e2m1x8(x[i][1]));
+      if ((g & 1) == 0) (i ? c.vs : c.ks)[at * (D / 32) + (g >> 1)] = static_cast<uint8_t>(byte);
+    }
+    if (at >= 0 && weights && g == 0) weights[at] = 0.f;
   });
 }
 
@@ -186,55 +181,47 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
-// read: one thread per 16 channels of a token's K and V, each written as one 32-byte sector.
+// read: one thread per scale block of a token's K and V, written as whole 32-byte sectors.
 // The output's bf16 values are the bound (4 of 5.06 bytes per value pair).
 template <int D>
 __global__ void __launch_bounds__(256)
 b2g_kv4_read_kernel(Kv4Cache c, Kv4Batch bt, const int* __restrict__ start, __nv_bfloat16* __restrict__ k,
                     __nv_bfloat16* __restrict__ v, int* status) {
-  constexpr int kPer = D / 16;
+  constexpr int kPer = D / 32;
   griddep_wait();
-  kv4_for_rows(bt.rows, c.heads * kPer, [&](const int (&row)[kRowsDeep], int in, const bool (&live)[kRowsDeep]) {
+  kv4_for_rows(bt.rows, c.heads * kPer, [&](int row, int in, bool live) {
+    if (!live) return;
     const int head = in / kPer, g = in % kPer;
-    long long at[kRowsDeep];
+    const int b = kv4_seq_of_row(bt, row);
+    int first, end;
+    kv4_rows(bt, b, first, end);
+    const long long token = static_cast<long long>(__ldg(start + b)) + row - first;
+    long long at = -1;
+    if (row >= first && row < end && token >= 0 && token < (static_cast<long long>(bt.width) << c.page_log2))
+      at = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, static_cast<int>(token), status);
+    uint4 codes[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    float s[2] = {0.f, 0.f};
+    if (at >= 0) {
 #pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n) {
-      at[n] = -1;
-      if (live[n]) {
-        const int b = kv4_seq_of_row(bt, row[n]);
-        int first, end;
-        kv4_rows(bt, b, first, end);
-        const long long token = static_cast<long long>(__ldg(start + b)) + row[n] - first;
-        if (row[n] >= first && row[n] < end && token >= 0 && token < (static_cast<long long>(bt.width) << c.page_log2))
-          at[n] = kv4_token(c, bt.table + static_cast<long long>(b) * bt.width, head, static_cast<int>(token), status);
+      for (int i = 0; i < 2; ++i) {
+        codes[i] = *(reinterpret_cast<const uint4*>((i ? c.v : c.k) + at * (D / 2)) + g);
+        s[i] = kv4_scale_value((i ? c.vs : c.ks)[at * (D / 32) + g]);
       }
     }
-    uint2 codes[kRowsDeep][2];
-    float s[kRowsDeep][2];
+    const long long to = (static_cast<long long>(row) * c.heads + head) * D + g * 32;
 #pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n)
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t word[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        codes[n][i] = make_uint2(0, 0);
-        s[n][i] = 0.f;
-        if (at[n] >= 0) {
-          codes[n][i] = *(reinterpret_cast<const uint2*>((i ? c.v : c.k) + at[n] * (D / 2)) + g);
-          s[n][i] = kv4_scale_value((i ? c.vs : c.ks)[at[n] * (D / 32) + (g >> 1)]);
-        }
-      }
-#pragma unroll
-    for (int n = 0; n < kRowsDeep; ++n) {
-      if (!live[n]) continue;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int half = 0; half < 2; ++half) {
         uint32_t w[8], x[4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (j % 4 == 0) e2m1x8_to_f16(j ? codes[n][i].y : codes[n][i].x, x);
+          if (j % 4 == 0) e2m1x8_to_f16(word[2 * half + j / 4], x);
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x[j % 4]));
-          w[j] = pack_bf16x2(y.x * s[n][i], y.y * s[n][i]);
+          w[j] = pack_bf16x2(y.x * s[i], y.y * s[i]);
         }
-        st_global_v8((i ? v : k) + (static_cast<long long>(row[n]) * c.heads + head) * D + g * 16, w);
+        st_global_v8((i ? v : k) + to + half * 16, w);
       }
     }
   });

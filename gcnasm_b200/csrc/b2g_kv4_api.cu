@@ -210,7 +210,7 @@ int b2g_kv4_append(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const
   if (rc) return rc;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const dim3 grid(row_grid(batch->rows, f.c.heads * (D / 8), f.sms));
+    const dim3 grid(row_grid(batch->rows, f.c.heads * (D / 16), f.sms));
     if (x_dtype == B2G_OUT_F32)
       rc = launch(b2g_kv4_append_kernel<float, D>, grid, 256, 0, f.st, f.c, f.bt, static_cast<const float*>(k),
                   static_cast<const float*>(v), k_row_stride, k_head_stride, v_row_stride, v_head_stride, weights, f.status);
@@ -230,7 +230,7 @@ int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const i
   if (rc) return rc;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    rc = launch(b2g_kv4_read_kernel<D>, dim3(row_grid(batch->rows, f.c.heads * (D / 16), f.sms)), 256, 0, f.st, f.c, f.bt, start,
+    rc = launch(b2g_kv4_read_kernel<D>, dim3(row_grid(batch->rows, f.c.heads * (D / 32), f.sms)), 256, 0, f.st, f.c, f.bt, start,
                 static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), f.status);
   });
   return rc;
