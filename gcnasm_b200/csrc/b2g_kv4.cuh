@@ -399,13 +399,15 @@ struct Kv4Piece {
   }
 };
 
-// To other pages, in any order: D / 16 lanes per token, a 16-byte piece each, the first lane
-// the scales and the weight too; a lane has four tokens in flight.
+// To other pages, in any order: D / 16 lanes per token, a 16-byte piece each; the first three
+// take the scales and the weight too.  Latency (kept number, two page numbers, codes) is hidden by
+// the warps of six blocks on an SM, with two tokens in flight in each lane.
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 b2g_kv4_move_kernel(Kv4Cache c, Kv4Batch bt, float* weights, int budget, const int* __restrict__ out_table,
                     int out_width, const int* __restrict__ kept, int* new_lens, int* status) {
-  constexpr int kLanes = D / 16, kTokens = 256 / kLanes, kDeep = 4;
+  constexpr int kLanes = D / 16, kTokens = 256 / kLanes, kDeep = 2;
+  using S = typename std::conditional<D == 64, uint16_t, typename std::conditional<D == 128, uint32_t, uint64_t>::type>::type;
   griddep_wait();
   const int h = blockIdx.y, b = blockIdx.z;
   // lens may be new_lens: this thread alone reads and writes it
@@ -414,38 +416,38 @@ b2g_kv4_move_kernel(Kv4Cache c, Kv4Batch bt, float* weights, int budget, const i
   const int* from_row = bt.table + static_cast<long long>(b) * bt.width;
   const int* to_row = out_table + static_cast<long long>(b) * out_width;
   const int* mine = kept + (static_cast<long long>(b) * c.heads + h) * budget;
-  for (int base = blockIdx.x * (kTokens * kDeep); base < budget; base += gridDim.x * (kTokens * kDeep)) {
-    int j[kDeep];
-    long long from[kDeep], to[kDeep];
-    Kv4Piece<D> p[kDeep], more[kDeep];
+  uint8_t* codes = piece < kLanes / 2 ? c.k + piece * 16 : c.v + (piece - kLanes / 2) * 16;
+  const int slot0 = blockIdx.x * (kTokens * kDeep) + sub;
+  int j[kDeep];
 #pragma unroll
-    for (int e = 0; e < kDeep; ++e) {
-      const int slot = base + e * kTokens + sub;
-      j[e] = slot < budget ? __ldg(mine + slot) : -1;
+  for (int e = 0; e < kDeep; ++e) j[e] = slot0 + e * kTokens < budget ? __ldg(mine + slot0 + e * kTokens) : -1;
+  long long from[kDeep], to[kDeep];
+#pragma unroll
+  for (int e = 0; e < kDeep; ++e) {
+    from[e] = to[e] = -1;
+    if (j[e] >= 0) {
+      from[e] = kv4_token(c, from_row, h, j[e], status);
+      to[e] = kv4_token(c, to_row, h, slot0 + e * kTokens, status);
     }
-#pragma unroll
-    for (int e = 0; e < kDeep; ++e) {
-      const int slot = base + e * kTokens + sub;
-      from[e] = to[e] = -1;
-      if (j[e] >= 0) {
-        from[e] = kv4_token(c, from_row, h, j[e], status);
-        to[e] = kv4_token(c, to_row, h, slot, status);
-      }
-      if (to[e] < 0) from[e] = -1;
-    }
-#pragma unroll
-    for (int e = 0; e < kDeep; ++e)
-      if (from[e] >= 0) {
-        p[e].load(c, weights, from[e], piece);
-        if (piece == 0) more[e].load(c, weights, from[e], kLanes);
-      }
-#pragma unroll
-    for (int e = 0; e < kDeep; ++e)
-      if (from[e] >= 0) {
-        p[e].store(c, weights, to[e], piece);
-        if (piece == 0) more[e].store(c, weights, to[e], kLanes);
-      }
+    if (to[e] < 0) from[e] = -1;
   }
+  uint4 x[kDeep];
+  S small[kDeep];
+  float w[kDeep];
+#pragma unroll
+  for (int e = 0; e < kDeep; ++e)
+    if (from[e] >= 0) {
+      x[e] = *reinterpret_cast<const uint4*>(codes + from[e] * (D / 2));
+      if (piece < 2) small[e] = *reinterpret_cast<const S*>((piece ? c.vs : c.ks) + from[e] * (D / 32));
+      else if (piece == 2) w[e] = weights[from[e]];
+    }
+#pragma unroll
+  for (int e = 0; e < kDeep; ++e)
+    if (from[e] >= 0) {
+      *reinterpret_cast<uint4*>(codes + to[e] * (D / 2)) = x[e];
+      if (piece < 2) *reinterpret_cast<S*>((piece ? c.vs : c.ks) + to[e] * (D / 32)) = small[e];
+      else if (piece == 2) weights[to[e]] = w[e];
+    }
 }
 
 // In place: one CTA per (sequence, kv head) moves the tokens in order, a batch at a time.

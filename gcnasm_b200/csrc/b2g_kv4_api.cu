@@ -321,7 +321,7 @@ int b2g_kv4_evict(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, float*
     if (in_place)
       rc = launch(b2g_kv4_move_in_place_kernel<D>, dim3(lists), 1024, 0, f.st, f.c, f.bt, weights, budget, kept, new_lens, f.status);
     else
-      rc = launch(b2g_kv4_move_kernel<D>, dim3((budget + 16384 / D - 1) / (16384 / D), f.c.heads, f.bt.seqs), 256, 0, f.st, f.c, f.bt,
+      rc = launch(b2g_kv4_move_kernel<D>, dim3((budget + 8192 / D - 1) / (8192 / D), f.c.heads, f.bt.seqs), 256, 0, f.st, f.c, f.bt,
                   weights, budget, out_table, out_width, kept, new_lens, f.status);
   });
   return rc;
