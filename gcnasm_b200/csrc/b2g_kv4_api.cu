@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 
 #include "b2g_host.h"
@@ -118,17 +119,20 @@ int launch(void (*kernel)(P...), dim3 grid, int block, size_t smem, cudaStream_t
 // CTAs of a decode kernel on an SM at most, which the workspace is sized for
 constexpr int decode_ctas(int nt) { return nt == 1 ? 4 : 2; }
 
-long long decode_workspace(int sms, int dim) {
-  long long most = 0;
+// The first bytes: which items were cut, 16 for each CTA; then two parts for each.  Kernels of one
+// call follow one another on the stream and share it.
+long long workspace_size(int sms, int dim) {
+  const long long prompt_rows = dim == 256 ? PromptCfg<256>::kRows : PromptCfg<128>::kRows;
+  long long most = sms * (16 + 2 * prompt_rows * (dim + 2) * 4);
   for (int nt : {1, 2, 4}) {
     const long long ctas = static_cast<long long>(sms) * decode_ctas(nt);
-    most = std::max(most, ctas * 16 + 2 * ctas * 8 * nt * (dim + 2) * 4);
+    most = std::max(most, ctas * (16 + 2 * 8 * nt * (dim + 2) * 4));
   }
   return most;
 }
 
 // From this many rows of a kv head on, the tcgen05 kernel
-constexpr long long kPromptRows = 64;
+constexpr int kPromptRows = 64;
 
 // Resident CTAs per SM, at most `most`, of a kernel with `smem` dynamic bytes on the current
 // device; 0: it does not fit.  Asked of the runtime once per kernel, device and size class.
@@ -150,7 +154,7 @@ int resident(K kernel, int block, size_t smem, int most, int dev, std::atomic<in
 }
 
 template <int D, int NT, bool kTwin>
-int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, void* workspace) {
+int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, int max_rows, void* workspace) {
   using Cfg = DecodeCfg<D, NT, kTwin>;
   static std::atomic<int> few[64], many[64];
   // room for the prefix sums of 512 sequences, or of as many as there can be
@@ -161,23 +165,26 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   const int grid = n * f.sms;
   int4* desc = static_cast<int4*>(workspace);
   float* partial = reinterpret_cast<float*>(desc + grid);
-  int rc = launch(b2g_kv4_decode_kernel<D, NT, kTwin>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, partial, desc, f.status);
+  int rc = launch(b2g_kv4_decode_kernel<D, NT, kTwin>, dim3(grid), 128, smem, f.st, f.c, f.bt, m, q, o, max_rows, partial, desc,
+                  f.status);
   if (rc) return rc;
   // blocks of four rows for items in many parts took 2 us more wherever most have nothing to join
   constexpr int kRB = std::min(Cfg::kRows, 16);
-  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, kRB>, dim3(grid, Cfg::kRows / kRB), 512, 0, f.st, f.bt, q, o, partial, desc);
+  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, kRB, false>, dim3(grid, Cfg::kRows / kRB), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
 template <int D, bool kCap>
-int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, long long group_rows) {
+int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, int min_rows, void* workspace) {
   using Cfg = PromptCfg<D>;
   static std::atomic<int> known[64];
   if (resident(b2g_kv4_prompt_kernel<D, kCap>, Cfg::kThreads, Cfg::kSmem, 1, f.dev, known) < 1)
     return host_fail(B2G_ERR_CUDA, "the prompt kernel does not fit on the device");
-  const long long blocks = (group_rows + Cfg::kRows - 1) / Cfg::kRows;
-  if (blocks > 65535) return host_fail(B2G_ERR_UNSUPPORTED, "max_new %lld x the heads of a group is beyond %d rows", group_rows, 65535 * Cfg::kRows);
-  return launch(b2g_kv4_prompt_kernel<D, kCap>, dim3(f.c.heads, f.bt.seqs, static_cast<unsigned>(blocks)), Cfg::kThreads, Cfg::kSmem,
-                f.st, f.c, f.bt, m, q, o, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
+  int4* desc = static_cast<int4*>(workspace);
+  float* partial = reinterpret_cast<float*>(desc + f.sms);
+  int rc = launch(b2g_kv4_prompt_kernel<D, kCap>, dim3(f.sms), Cfg::kThreads, Cfg::kSmem, f.st, f.c, f.bt, m, q, o, min_rows, partial,
+                  desc, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
+  if (rc) return rc;
+  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, 16, true>, dim3(f.sms, Cfg::kRows / 16), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
 template <int D>
@@ -241,7 +248,7 @@ long long b2g_kv4_workspace_bytes(int head_dim) {
     return -host_fail(B2G_ERR_UNSUPPORTED, "head_dim %d is not 64, 128 or 256", head_dim);
   int sms = 0, *status = nullptr;
   const int rc = host_device(&sms, &status);
-  return rc ? -rc : decode_workspace(sms, head_dim);
+  return rc ? -rc : workspace_size(sms, head_dim);
 }
 
 int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask, const void* q,
@@ -254,20 +261,26 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   if ((rc = check_queries(cache, mask, q, q_row_stride, q_head_stride, heads, "q"))) return rc;
   if ((rc = check_queries(cache, mask, out, out_row_stride, out_head_stride, heads, "out"))) return rc;
   if (!lse || !aligned(lse, 4)) return host_fail(B2G_ERR_INVALID_ARG, "null or misaligned lse");
-  const long long need = decode_workspace(f.sms, f.dim);
+  const long long need = workspace_size(f.sms, f.dim);
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
     return host_fail(B2G_ERR_WORKSPACE, "the workspace holds %lld bytes, not %lld (16-byte aligned)", workspace_bytes, need);
   const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
   const Kv4Out o{static_cast<__nv_bfloat16*>(out), out_row_stride, out_head_stride, lse};
   const long long rows = static_cast<long long>(std::max(1, batch->cu ? std::min(batch->max_new, batch->rows) : 1)) * qs.group;
+  // Prompts and single tokens in one batch: each kernel takes its own sequences.  Where the others are
+  // prompts too, judged by their average, one launch serves; what it serves is the same either way.
+  const bool mixed = f.bt.seqs > 1 && (batch->rows - batch->max_new) * static_cast<long long>(qs.group) < 4 * kPromptRows * (f.bt.seqs - 1);
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (rows >= kPromptRows) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, rows) : prompt<D, false>(f, m, qs, o, rows);
-    else if (rows <= 4) rc = decode<D, 1, true>(f, m, qs, o, workspace);
-    else if (rows <= 8) rc = decode<D, 1, false>(f, m, qs, o, workspace);
-    else if (rows <= 16 || D == 256) rc = decode<D, 2, false>(f, m, qs, o, workspace);
-    else if constexpr (D < 256) rc = decode<D, 4, false>(f, m, qs, o, workspace);
+    const int limit = rows < kPromptRows ? INT_MAX : mixed ? static_cast<int>(kPromptRows) : 0;  // rows from which the prompt kernel takes a sequence
+    if (limit != INT_MAX) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, limit, workspace) : prompt<D, false>(f, m, qs, o, limit, workspace);
+    if (limit == 0 || rc) return;
+    const long long here = std::min<long long>(rows, limit);
+    if (here <= 4) rc = decode<D, 1, true>(f, m, qs, o, limit, workspace);
+    else if (here <= 8) rc = decode<D, 1, false>(f, m, qs, o, limit, workspace);
+    else if (here <= 16 || D == 256) rc = decode<D, 2, false>(f, m, qs, o, limit, workspace);
+    else if constexpr (D < 256) rc = decode<D, 4, false>(f, m, qs, o, limit, workspace);
   });
   return rc;
 }

@@ -287,19 +287,21 @@ struct Kv4Walk {
   int blocks;  // row blocks of the sequence
 };
 
-// Two channels of a finished row.  Position 16 i + 2 g + e of a row of O, as the warps keep it
-// (pair = 8 i + g), is channel 32 (i / 2) + 4 g + 2 (i % 2) + e.
+// Two channels of a finished row.  Position 16 i + 2 g + e of a row of O, as the decode kernel's
+// warps keep it (pair = 8 i + g), is channel 32 (i / 2) + 4 g + 2 (i % 2) + e; kPlain: channels in order.
+template <bool kPlain>
 __device__ __forceinline__ void kv4_finish(const Kv4Out& out, long long row, int head, int heads, int pair, float2 v, float m,
                                            float l) {
   const float f = l == 0.f ? 0.f : kTwo64 / l;
-  const int ch = 32 * (pair >> 4) + 4 * (pair & 7) + 2 * ((pair >> 3) & 1);
+  const int ch = kPlain ? 2 * pair : 32 * (pair >> 4) + 4 * (pair & 7) + 2 * ((pair >> 3) & 1);
   *reinterpret_cast<uint32_t*>(out.out + row * out.row + head * out.head + ch) = pack_bf16x2(v.x * f, v.y * f);
   if (pair == 0) out.lse[row * heads + head] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
+// Sequences with fewer than max_rows query rows of a kv head.
 template <int D, int NT, bool kTwin>
 __global__ void __launch_bounds__(128, NT == 1 && D < 256 ? 3 : 2)
-b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, float* __restrict__ partial,
+b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, int max_rows, float* __restrict__ partial,
                       int4* __restrict__ desc, int* status) {
   using Cfg = DecodeCfg<D, NT, kTwin>;
   constexpr int kRows = Cfg::kRows, kPad = Cfg::kPad, kChunks = Cfg::kChunks, kStages = Cfg::kStages;
@@ -323,6 +325,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 
   kv4_scan(bt.seqs, s_pre, s_scan, [&](int b) {
     const Kv4Span s = kv4_span(bt, mask, b, c.page_log2);
+    if (s.rows * q.group >= max_rows) return 0ll;
     return static_cast<long long>(s.units) * c.heads * ((s.rows * q.group + kRows - 1) / kRows);
   });
   const long long total = s_pre[bt.seqs];
@@ -681,7 +684,7 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         if (whole) {
           const long long row = ps.first + (r0 + r) / q.group;
           const int head = ph * q.group + (r0 + r) % q.group;
-          kv4_finish(out, row, head, q.heads, pair, v, top, sum);
+          kv4_finish<false>(out, row, head, q.heads, pair, v, top, sum);
         } else {
           *reinterpret_cast<float2*>(slot + r * D + 2 * pair) = v;
           if (pair == 0) {
@@ -705,8 +708,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
 }
 
 // Joins the parts of an item that was cut: block (i, y) has kRB rows from kRB y on of the item that
-// decode CTA i began.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
-template <int D, int kRows, int kRB>
+// CTA i began.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
+template <int D, int kRows, int kRB, bool kPlain>
 __global__ void __launch_bounds__(512)
 b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial, const int4* __restrict__ desc) {
   constexpr int kE = D / 32, kShare = 16 / kRB;
@@ -785,7 +788,7 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
   const long long row = first + (r0 + r) / q.group;
   const int head = h * q.group + (r0 + r) % q.group;
 #pragma unroll
-  for (int e = 0; e < kE; e += 2) kv4_finish(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), t, sum);
+  for (int e = 0; e < kE; e += 2) kv4_finish<kPlain>(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), t, sum);
 }
 
 }  // namespace b2g

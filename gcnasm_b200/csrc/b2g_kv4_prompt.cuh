@@ -7,13 +7,15 @@
 //   P = 2^(S - m)    one thread per row; P as two bf16 terms over S in TMEM
 //   O += P V         tcgen05.mma, P from TMEM, V in shared memory with channels along its rows
 // Warps: one softmax warpgroup per query tile, four warps that turn codes into bf16 tiles, one
-// that issues the products.
+// that issues the products (and three that fill its warpgroup, whose registers the others take).
 //
 // What bounds it: for D = 128 the products of a step take 3072 clocks at 4096 multiplications a
 // clock, its 2 x 128 x 128 exponentials 2048 at 16 a clock, decoding 32768 codes ~700 issue slots a
 // scheduler.  Hence two query tiles: while one's S is being exponentiated the other's products
 // run, and what a step decodes serves 256 rows.  D = 256 leaves TMEM for one query tile, whose S
-// has two buffers instead.
+// has two buffers instead.  The items' steps, laid end to end, are cut evenly among one CTA on each
+// SM (whole waves of items left 15 % of the GPU idle at the end of 256 items, and most of it where
+// there are few); parts of a cut item are joined by a second kernel, as in the decode kernel.
 //
 // Codes become bf16 as in the decode kernel (times 2^-64, exact), in the order 0 4 1 5 2 6 3 7 of
 // each eight channels: Q is stored in the same order, O's columns are put back when written.
@@ -33,14 +35,22 @@ struct PromptCfg {
   static constexpr int kN = D == 256 ? 64 : 128;  // cached tokens of a step
   static constexpr int kSB = D == 256 ? 2 : 1;    // buffers of a query tile's S
   static constexpr int kRows = 128 * kNQ;
-  static constexpr int kThreads = kNQ * 128 + 128 + 32;
+  static constexpr int kThreads = kNQ * 128 + 256;
+  // registers of a thread of the softmax, decoding and product warpgroups: together what the block is
+  // launched with (128 a thread, or 168)
+  static constexpr int kRegsSoftmax = D == 256 ? 216 : 160;
+  static constexpr int kRegsDecode = D == 256 ? 152 : 104;
+  static constexpr int kRegsProduct = D == 256 ? 136 : 88;
+  static_assert(kNQ * kRegsSoftmax + kRegsDecode + kRegsProduct <= (D == 256 ? 3 * 168 : 4 * 128), "a larger sum would wait forever");
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kKBytes = kN * D * 2;
   static constexpr int kOffK = kNQ * kQBytes;
   static constexpr int kOffV = kOffK + 2 * kKBytes;
   static constexpr int kOffBar = kOffV + 2 * kKBytes;
-  static constexpr int kBars = 1 + 8 + 2 * kNQ * kSB + 2 * kNQ + 1;
+  static constexpr int kBars = 8 + 2 * kNQ * kSB + 3 * kNQ + 1;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;  // and room to align to 1024
+  // An item is cut into no less than this on average: a piece starts and ends in about two steps' time.
+  static constexpr int kMinSteps = 4;
   static constexpr uint32_t kColO = 256;  // S at column (tile * kSB + buffer) * kN, O here
 };
 
@@ -153,23 +163,118 @@ __device__ __forceinline__ uint32_t kv4_bits(int a, int b) {
   return below_b & ~below_a;
 }
 
+// A CTA's piece of work: n steps from step s0 of an item (sequence, kv head, block of query rows).
+struct Kv4PromptPiece {
+  int b, h, blk, blocks;
+  int first, rows, len, group_rows;  // of the sequence
+  int j0, steps;                     // of the item: its first step's number and how many it has
+  int s0, n;                         // of the piece; n = 0 where no row of the item sees a token
+  long long u;                       // its first unit among all
+};
+
+template <int D>
+__device__ __forceinline__ void kv4_prompt_seq(Kv4PromptPiece& w, const Kv4Batch& bt, const Kv4Queries& q, int page_log2,
+                                               int min_rows) {
+  int end;
+  kv4_rows(bt, w.b, w.first, end);
+  w.rows = end - w.first;
+  w.len = kv4_len(bt, w.b, page_log2);
+  w.group_rows = w.rows * q.group;
+  w.blocks = w.group_rows < min_rows ? 0 : (w.group_rows + PromptCfg<D>::kRows - 1) / PromptCfg<D>::kRows;
+}
+
+template <int D>
+__device__ __forceinline__ void kv4_prompt_item(Kv4PromptPiece& w, const Kv4Mask& m, const Kv4Queries& q) {
+  const int r0 = w.blk * PromptCfg<D>::kRows, r1 = min(r0 + PromptCfg<D>::kRows, w.group_rows) - 1;
+  int lo0, hi1, unused;
+  kv4_visible(m, w.len - w.rows + r0 / q.group, w.len, lo0, unused);
+  kv4_visible(m, w.len - w.rows + r1 / q.group, w.len, unused, hi1);
+  w.j0 = lo0 / PromptCfg<D>::kN;
+  w.steps = max(0, (hi1 + PromptCfg<D>::kN - 1) / PromptCfg<D>::kN - w.j0);
+}
+
+// An item's units of work: its steps, one where it has none.
+template <int D>
+__device__ __forceinline__ int kv4_prompt_units(Kv4PromptPiece& w, int blk, const Kv4Mask& m, const Kv4Queries& q) {
+  w.blk = blk;
+  kv4_prompt_item<D>(w, m, q);
+  return max(1, w.steps);
+}
+
+__device__ __forceinline__ long long warp_sum(long long x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ long long warp_scan(long long x, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += v;
+  }
+  return x;
+}
+
+// Units of sequences [b0, b1), by a warp.  Where one of them has unit `find` of the numbering that
+// begins at `before`: found = it, the unit's number in it and the units of one of its kv heads.
+struct Kv4Found {
+  int b;
+  long long unit, per_head;
+};
+template <int D>
+__device__ __forceinline__ long long kv4_prompt_scan(const Kv4Batch& bt, const Kv4Mask& m, const Kv4Queries& q, int page_log2, int min_rows,
+                                                     int heads, int b0, int b1, long long before, long long find, Kv4Found* found) {
+  const int lane = threadIdx.x & 31;
+  Kv4PromptPiece w;
+  long long sum = 0;
+  for (int base = b0; base < b1; base += 32) {
+    w.b = base + lane;
+    w.blocks = 0;
+    if (w.b < b1) kv4_prompt_seq<D>(w, bt, q, page_log2, min_rows);
+    long long units = 0;  // of one kv head: a few items by the sequence's lane, many by the warp
+    if (w.blocks <= 4)
+      for (int i = 0; i < w.blocks; ++i) units += kv4_prompt_units<D>(w, i, m, q);
+    for (unsigned many = __ballot_sync(0xffffffffu, w.blocks > 4); many; many &= many - 1) {
+      const int from = __ffs(many) - 1;
+      Kv4PromptPiece x;
+      x.b = base + from;
+      kv4_prompt_seq<D>(x, bt, q, page_log2, min_rows);
+      long long part = 0;
+      for (int i = lane; i < x.blocks; i += 32) part += kv4_prompt_units<D>(x, i, m, q);
+      part = warp_sum(part);
+      if (lane == from) units = part;
+    }
+    const long long mine = units * heads, upto = before + sum + warp_scan(mine, lane);
+    if (found && mine && upto - mine <= find && find < upto) *found = {w.b, find - (upto - mine), units};
+    sum += warp_sum(mine);
+  }
+  return sum;
+}
+
+// Sequences with at least min_rows query rows of a kv head.
 template <int D, bool kCap>
 __global__ void __launch_bounds__(PromptCfg<D>::kThreads, 1)
-b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, uint64_t timeout_ns, int* status) {
+b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, int min_rows, float* __restrict__ partial,
+                      int4* __restrict__ desc, uint64_t timeout_ns, int* status) {
   using Cfg = PromptCfg<D>;
   constexpr int kNQ = Cfg::kNQ, kN = Cfg::kN, kSB = Cfg::kSB;
   extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_scan[Cfg::kThreads / 32];
+  __shared__ Kv4Found s_found;
+  // each warp's piece: kept here, not in registers, which the loops over S need
+  __shared__ Kv4PromptPiece s_piece[Cfg::kThreads / 32];
+  __shared__ long long s_u0, s_u1, s_total, s_ctas;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;
-  uint64_t* k_empty = bars + 3;
-  uint64_t* v_full = bars + 5;
-  uint64_t* v_empty = bars + 7;
-  uint64_t* s_full = bars + 9;                // [tile][buffer]
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + 2;
+  uint64_t* v_full = bars + 4;
+  uint64_t* v_empty = bars + 6;
+  uint64_t* s_full = bars + 8;                // [tile][buffer]
   uint64_t* p_full = s_full + kNQ * kSB;
-  uint64_t* o_done = p_full + kNQ * kSB;      // [tile]: a step's O
-  uint64_t* o_last = o_done + kNQ;            // [tile]: the last step's
+  uint64_t* q_full = p_full + kNQ * kSB;      // [tile]: a piece's Q
+  uint64_t* o_done = q_full + kNQ;            // [tile]: a step's O
+  uint64_t* o_last = o_done + kNQ;            // [tile]: a piece's last step's
   uint64_t* fin = o_last + kNQ;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -177,22 +282,84 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   constexpr int kDecodeWarp = 4 * kNQ, kMmaWarp = kDecodeWarp + 4;
 
   griddep_wait();
-  const int h = blockIdx.x, b = blockIdx.y;
-  int first, end;
-  kv4_rows(bt, b, first, end);
-  const int rows = end - first, len = kv4_len(bt, b, c.page_log2), group_rows = rows * q.group;
-  // the last blocks see most: they come first
-  const int blk = (group_rows + Cfg::kRows - 1) / Cfg::kRows - 1 - static_cast<int>(blockIdx.z);
-  if (blk < 0) return;
-  const int r0 = blk * Cfg::kRows, r1 = min(r0 + Cfg::kRows, group_rows) - 1;
-  int lo0, hi1, unused;
-  kv4_visible(mask, len - rows + r0 / q.group, len, lo0, unused);
-  kv4_visible(mask, len - rows + r1 / q.group, len, unused, hi1);
-  const int j0 = lo0 / kN, steps = max(0, (hi1 + kN - 1) / kN - j0);
-  const int* pages = bt.table + static_cast<long long>(b) * bt.width;
+  // ---- work: all items' units end to end, cut evenly among the CTAs
+  const int me = blockIdx.x;
+  if (threadIdx.x == 0) desc[me] = make_int4(0, 0, 0, 0);
+  {
+    constexpr int kWarps = Cfg::kThreads / 32;
+    const int per = (bt.seqs + kWarps - 1) / kWarps, b0 = min(warp * per, bt.seqs), b1 = min(b0 + per, bt.seqs);
+    const long long mine = kv4_prompt_scan<D>(bt, mask, q, c.page_log2, min_rows, c.heads, b0, b1, 0, 0, nullptr);
+    if (lane == 0) s_scan[warp] = mine;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) before += s_scan[i];
+      total += s_scan[i];
+    }
+    const long long ctas = min(static_cast<long long>(gridDim.x), max(total / Cfg::kMinSteps, min(total, 1ll)));
+    if (me >= ctas) return;
+    const long long u = total * me / ctas;
+    if (threadIdx.x == 0) {
+      s_u0 = u;
+      s_u1 = total * (me + 1) / ctas;
+      s_total = total;
+      s_ctas = ctas;
+    }
+    if (before <= u && u < before + mine) {  // this warp's sequences have the first unit
+      kv4_prompt_scan<D>(bt, mask, q, c.page_log2, min_rows, c.heads, b0, b1, before, u, &s_found);
+      __syncwarp();
+      Kv4PromptPiece w;
+      w.b = s_found.b;
+      w.u = u;
+      kv4_prompt_seq<D>(w, bt, q, c.page_log2, min_rows);
+      w.h = static_cast<int>(s_found.unit / s_found.per_head);
+      long long rest = s_found.unit - w.h * s_found.per_head;
+      for (int base = 0;; base += 32) {  // its item of the kv head
+        const int units = base + lane < w.blocks ? kv4_prompt_units<D>(w, base + lane, mask, q) : 0;
+        const long long upto = warp_scan(units, lane);
+        if (upto - units <= rest && rest < upto) {
+          w.s0 = static_cast<int>(rest - (upto - units));
+          s_piece[0] = w;
+        }
+        const long long all = __shfl_sync(0xffffffffu, upto, 31);
+        if (rest < all) break;
+        rest -= all;
+      }
+    }
+    __syncthreads();
+    Kv4PromptPiece w = s_piece[0];
+    w.n = static_cast<int>(min(static_cast<long long>(w.steps - (w.steps ? w.s0 : 0)), s_u1 - u));
+    __syncthreads();
+    if (lane == 0) s_piece[warp] = w;
+    __syncwarp();
+  }
+  const Kv4PromptPiece& w = s_piece[warp];
+  const long long u1 = s_u1;
+  // the next piece, where one is left
+  auto go_on = [&]() {
+    Kv4PromptPiece x = w;
+    x.u += max(1, x.n);
+    if (x.u < u1) {
+      x.s0 = 0;
+      if (++x.blk >= x.blocks) {
+        x.blk = 0;
+        if (++x.h >= c.heads) {
+          x.h = 0;
+          do {
+            ++x.b;
+            kv4_prompt_seq<D>(x, bt, q, c.page_log2, min_rows);
+          } while (x.blocks == 0);
+        }
+      }
+      kv4_prompt_item<D>(x, mask, q);
+      x.n = static_cast<int>(min(static_cast<long long>(x.steps), u1 - x.u));
+    }
+    __syncwarp();
+    if (lane == 0) s_piece[warp] = x;
+    __syncwarp();
+  };
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, kNQ * 128);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 128);
       mbar_init(&v_full[i], 128);
@@ -204,6 +371,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       mbar_init(&p_full[i], 128);
     }
     for (int i = 0; i < kNQ; ++i) {
+      mbar_init(&q_full[i], 128);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_last[i], 1);
     }
@@ -216,14 +384,30 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  // Barrier phases are counted over the CTA's whole work: `g0` steps and `np` pieces with steps so far.
+  bool ok = true;
+  int g0 = 0, np = 0;
 
   if (warp < kDecodeWarp) {
     // ---------------------------------------------------------------- softmax: one thread per row
+    setmaxnreg_inc<Cfg::kRegsSoftmax>();
     const int tile = warp >> 2, in_tile = threadIdx.x & 127;
-    const int r = r0 + tile * 128 + in_tile;
-    const bool real = r < group_rows;
-    const int row = first + r / q.group, head = h * q.group + r % q.group;
-    {  // Q, in the codes' channel order; a negative scale goes to its signs
+    const float scale = fabsf(mask.scale) * kTwo64;
+    // with a cap: tanh's argument.  Not zero, so that -inf stays that
+    const float s_scale = fmaxf(kCap ? scale / mask.softcap : scale * kLog2e, 1.2e-38f);
+    const float cap2 = kCap ? mask.softcap * kLog2e : 0.f;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_at = tmem + lanes + Cfg::kColO + tile * D;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {  // all lanes go on, or none: what follows is the warp's
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, kDevTimeoutEpilogue, timeout_ns)) != 0;
+    };
+    while (w.u < u1 && ok) {
+    const int r0 = w.blk * Cfg::kRows, r = r0 + tile * 128 + in_tile;
+    const bool real = r < w.group_rows;
+    const int row = w.first + r / q.group, head = w.h * q.group + r % q.group;
+    const int* pages = bt.table + static_cast<long long>(w.b) * bt.width;
+    const int n = w.n, t0 = (w.j0 + w.s0) * kN, len = w.len;
+    if (n) {  // Q, in the codes' channel order; a negative scale goes to its signs
       const uint32_t flip = mask.scale < 0.f ? 0x80008000u : 0u;
       uint8_t* dst = smem + tile * Cfg::kQBytes + in_tile * 128;
       const uint4* src = reinterpret_cast<const uint4*>(q.q + row * q.q_row + head * q.q_head);
@@ -236,22 +420,13 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         *reinterpret_cast<uint4*>(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (in_tile & 7)) << 4)) = x;
       }
       fence_proxy_async_smem();
-      mbar_arrive(q_full);
+      mbar_arrive(&q_full[tile]);
     }
     int lo, hi;
-    kv4_visible(mask, len - rows + r / q.group, len, lo, hi);
-    const float scale = fabsf(mask.scale) * kTwo64;
-    // with a cap: tanh's argument.  Not zero, so that -inf stays that
-    const float s_scale = fmaxf(kCap ? scale / mask.softcap : scale * kLog2e, 1.2e-38f);
-    const float cap2 = kCap ? mask.softcap * kLog2e : 0.f;
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    float m = -1e30f, l0 = 0.f, l1 = 0.f;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {  // all lanes go on, or none: what follows is the warp's
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, kDevTimeoutEpilogue, timeout_ns)) != 0;
-    };
-    for (int i = 0; i < steps && ok; ++i) {
-      const int tb = (j0 + i) * kN;
+    kv4_visible(mask, w.len - w.rows + r / q.group, w.len, lo, hi);
+    float m = kNoMax, l0 = 0.f, l1 = 0.f;
+    for (int i = 0; i < n && ok; ++i) {
+      const int g = g0 + i, tb = t0 + i * kN;
       // which groups of 16 tokens have a page
       uint32_t there;
       {
@@ -260,10 +435,9 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         if (lane < kN / 16 && token < len) t = static_cast<unsigned>(__ldg(pages + (token >> c.page_log2))) < static_cast<unsigned>(c.pages);
         there = __ballot_sync(0xffffffffu, t);
       }
-      const int buf = kSB == 2 ? i & 1 : 0;
-      const uint32_t parity = kSB == 2 ? (i >> 1) & 1 : i & 1;
+      const int buf = kSB == 2 ? g & 1 : 0;
+      const uint32_t parity = kSB == 2 ? (g >> 1) & 1 : g & 1;
       const uint32_t s_at = tmem + lanes + (tile * kSB + buf) * kN;
-      const uint32_t o_at = tmem + lanes + Cfg::kColO + tile * D;
       const bool masked = __any_sync(0xffffffffu, tb < lo || tb + kN > hi) || there != (1u << (kN / 16)) - 1u;
       if (!(ok = wait(&s_full[tile * kSB + buf], parity))) break;
       tc_fence_after();
@@ -283,9 +457,9 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         m = fresh && need ? top : m + up;
         l0 *= f;
         l1 *= f;
-        // one buffer of S: step i's products came after step i - 1's in the pipe.  Two: they may have
-        // come before, but after step i - 2's, so the barrier is in phase i - 1 or just past it
-        if (kSB == 2 && i > 0 && !(ok = wait(&o_done[tile], (i - 1) & 1))) return;
+        // one buffer of S: step g's products came after step g - 1's in the pipe.  Two: they may have
+        // come before, but after step g - 2's, so the barrier is in phase g - 1 or just past it
+        if (kSB == 2 && i > 0 && !(ok = wait(&o_done[tile], (g - 1) & 1))) return;
         tc_fence_after();
 #pragma unroll 1
         for (int col = 0; i > 0 && col < D; col += 32) {
@@ -383,48 +557,59 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       tc_fence_before();
       mbar_arrive(&p_full[tile * kSB + buf]);
     }
-    // ---- output
+    // ---- output, or this piece's part of it
     const float l = l0 + l1;
-    if (steps > 0 && ok) ok = wait(&o_last[tile], 0);
+    const bool whole = w.s0 == 0 && n == w.steps;
+    if (n && ok) ok = wait(&o_last[tile], np & 1);
     if (ok) {
       tc_fence_after();
       const float f = l == 0.f ? 0.f : kTwo64 / l;
       uint8_t* dst = reinterpret_cast<uint8_t*>(out.out + row * out.row + head * out.head);
+      float* part = partial + (2ll * me + (w.u == s_u0 ? 0 : 1)) * (Cfg::kRows * (D + 2));
 #pragma unroll 1
       for (int col = 0; col < D; col += 32) {
         uint32_t x[32];
-        if (steps > 0) {
-          tmem_ld_32x32b_x32(tmem + lanes + Cfg::kColO + tile * D + col, x);
+        if (n) {
+          tmem_ld_32x32b_x32(o_at + col, x);
           tc_wait_ld();
         }
+        if (!real) continue;
+        // columns 0 .. 7 hold channels 0 4 1 5 2 6 3 7
+        if (whole) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[e]) * f);
-        if (real) {
+          for (int e = 0; e < 32; ++e) x[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[e]) * f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // columns 0 .. 7 hold channels 0 4 1 5 2 6 3 7
+          for (int i = 0; i < 4; ++i) {
             auto two = [&](int a, int d) { return pack_bf16x2(__uint_as_float(x[8 * i + a]), __uint_as_float(x[8 * i + d])); };
             *reinterpret_cast<uint4*>(dst + (col + 8 * i) * 2) = make_uint4(two(0, 2), two(4, 6), two(1, 3), two(5, 7));
           }
+        } else {
+          uint4* to = reinterpret_cast<uint4*>(part + (r - r0) * D + col);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            to[2 * i] = make_uint4(x[8 * i], x[8 * i + 2], x[8 * i + 4], x[8 * i + 6]);
+            to[2 * i + 1] = make_uint4(x[8 * i + 1], x[8 * i + 3], x[8 * i + 5], x[8 * i + 7]);
+          }
         }
       }
-      if (real) out.lse[static_cast<long long>(row) * q.heads + head] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+      if (real && whole) out.lse[static_cast<long long>(row) * q.heads + head] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+      if (real && !whole) *reinterpret_cast<float2*>(part + Cfg::kRows * D + 2 * (r - r0)) = make_float2(m, l);
+      if (!whole && w.s0 == 0 && threadIdx.x == 0) {
+        // this CTA begins the item; the ones after it, up to the one with its last unit, go on
+        const long long other = ((w.u + w.steps) * s_ctas - 1) / s_total;
+        desc[me] = make_int4(static_cast<int>(other) - me + 1, w.b, w.h * w.blocks + w.blk, w.u == s_u0 ? 0 : 1);
+      }
+    }
+    if (n) ++np;
+    g0 += n;
+    go_on();
     }
   } else if (warp < kMmaWarp) {
     // ---------------------------------------------------------------- codes to bf16 tiles
+    setmaxnreg_dec<Cfg::kRegsDecode>();
     // K of a step, then V, by the same code: halves are fetched one ahead, page numbers a step ahead
     constexpr int kWords = D == 64 ? 8 : 16;  // a thread's words of a half
     const int dt = threadIdx.x - kDecodeWarp * 32, tok = dt % kN, part = dt / kN;  // a warp's lanes: consecutive tokens
-    auto page_of = [&](int i) {
-      const int token = (j0 + i) * kN + tok;
-      return i < steps && token < len ? __ldg(pages + (token >> c.page_log2)) : -2;
-    };
-    // a step's token among all, -1 where it is not there
-    auto token_of = [&](int i, int page) {
-      const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
-      if (!there && page != -2) atomicCAS(status, 0, kDevBadPage);
-      const int token = (j0 + i) * kN + tok;
-      return there ? ((static_cast<long long>(page) * c.heads + h) << c.page_log2) + (token & ((1 << c.page_log2) - 1)) : -1ll;
-    };
     auto fetch = [&](uint4 (&x)[kWords / 4], uint32_t& scales, const uint8_t* codes, const uint8_t* bytes, long long at) {
       scales = 0;
 #pragma unroll
@@ -435,24 +620,37 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       if constexpr (D == 64) scales = *reinterpret_cast<const uint16_t*>(bytes + at * 2);
       else scales = *(reinterpret_cast<const uint32_t*>(bytes + at * (D / 32)) + part);
     };
-    bool ok = true;
+    while (w.u < u1 && ok) {
+    const int n_steps = w.n, t0 = (w.j0 + w.s0) * kN, len = w.len, h = w.h;
+    const int* pages = bt.table + static_cast<long long>(w.b) * bt.width;
+    auto page_of = [&](int i) {
+      const int token = t0 + i * kN + tok;
+      return i < n_steps && token < len ? __ldg(pages + (token >> c.page_log2)) : -2;
+    };
+    // a step's token among all, -1 where it is not there
+    auto token_of = [&](int i, int page) {
+      const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(c.pages);
+      if (!there && page != -2) atomicCAS(status, 0, kDevBadPage);
+      const int token = t0 + i * kN + tok;
+      return there ? ((static_cast<long long>(page) * c.heads + h) << c.page_log2) + (token & ((1 << c.page_log2) - 1)) : -1ll;
+    };
     uint4 now[kWords / 4], next[kWords / 4];
     uint32_t now_s, next_s;
     int page = page_of(0);
-    long long at = steps > 0 ? token_of(0, page) : -1;
+    long long at = n_steps ? token_of(0, page) : -1;
     fetch(now, now_s, c.k, c.ks, at);
     page = page_of(1);
 #pragma unroll 1
-    for (int i2 = 0; i2 < 2 * steps && ok; ++i2) {
-      const int i = i2 >> 1, st = i & 1;
+    for (int i2 = 0; i2 < 2 * n_steps && ok; ++i2) {
+      const int i = i2 >> 1, st = (g0 + i) & 1;
       const bool is_v = i2 & 1;
       if (is_v) {
-        at = i + 1 < steps ? token_of(i + 1, page) : -1;
+        at = i + 1 < n_steps ? token_of(i + 1, page) : -1;
         page = page_of(i + 2);
       }
       fetch(next, next_s, is_v ? c.k : c.v, is_v ? c.ks : c.vs, at);
       uint64_t* empty = is_v ? &v_empty[st] : &k_empty[st];
-      if (!mbar_wait(empty, ((i >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
+      if (!mbar_wait(empty, (((g0 + i) >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
       // a thread's channels of one token: words of eight codes to 16-byte pieces of 128-byte swizzled rows
       uint8_t* tile = smem + (is_v ? Cfg::kOffV : Cfg::kOffK) + st * Cfg::kKBytes + tok * 128;
       uint32_t even, odd;
@@ -475,68 +673,82 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       for (int n = 0; n < kWords / 4; ++n) now[n] = next[n];
       now_s = next_s;
     }
+    g0 += n_steps;
+    go_on();
+    }
   } else {
     // ---------------------------------------------------------------- products
-    if (lane == 0 && steps > 0) {
+    setmaxnreg_dec<Cfg::kRegsProduct>();
+    if (warp == kMmaWarp) {
       constexpr uint32_t kIdQK = idesc_bf16(128, kN, 0), kIdPV = idesc_bf16(128, D, 1);
-      auto qk = [&](int tile, int i) {
-        const uint32_t d = tmem + (tile * kSB + (kSB == 2 ? i & 1 : 0)) * kN;
-        const uint32_t a = smem_u32(smem + tile * Cfg::kQBytes), bk = smem_u32(smem + Cfg::kOffK + (i & 1) * Cfg::kKBytes);
+      auto qk = [&](int tile, int g) {  // of step g
+        const uint32_t d = tmem + (tile * kSB + (kSB == 2 ? g & 1 : 0)) * kN;
+        const uint32_t a = smem_u32(smem + tile * Cfg::kQBytes), bk = smem_u32(smem + Cfg::kOffK + (g & 1) * Cfg::kKBytes);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           mma_bf16_ss(d, desc_kmajor_sw128(a + (k >> 2) * (128 * 128) + (k & 3) * 32),
                       desc_kmajor_sw128(bk + (k >> 2) * (kN * 128) + (k & 3) * 32), kIdQK, k > 0);
       };
-      auto pv = [&](int tile, int i) {
-        const uint32_t a = tmem + (tile * kSB + (kSB == 2 ? i & 1 : 0)) * kN, d = tmem + Cfg::kColO + tile * D;
-        const uint32_t bv = smem_u32(smem + Cfg::kOffV + (i & 1) * Cfg::kKBytes);
+      auto pv = [&](int tile, int g, bool more) {  // more: onto what O holds
+        const uint32_t a = tmem + (tile * kSB + (kSB == 2 ? g & 1 : 0)) * kN, d = tmem + Cfg::kColO + tile * D;
+        const uint32_t bv = smem_u32(smem + Cfg::kOffV + (g & 1) * Cfg::kKBytes);
         // channels along the rows: 64 of them in 128 bytes, the next 64 kN rows on; eight tokens a kilobyte.
         // P: 32 tokens' first terms in 16 columns, their second terms in the next 16
 #pragma unroll
         for (int k = 0; k < kN / 16; ++k) {
           const uint64_t bd = smem_desc(bv + k * 2048, kN * 128, 1024, kLayoutSW128);
           const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;
-          mma_bf16_ts(d, ak, bd, kIdPV, i > 0 || k > 0);
+          mma_bf16_ts(d, ak, bd, kIdPV, more || k > 0);
           mma_bf16_ts(d, ak + 16, bd, kIdPV, 1);
         }
       };
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, status, kDevTimeoutMma, timeout_ns); };
-      bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
-      if (ok) {
-        for (int tile = 0; tile < kNQ; ++tile) {
-          qk(tile, 0);
-          tc_commit(&s_full[tile * kSB]);
-        }
-        tc_commit(&k_empty[0]);
-      }
-      for (int i = 0; i < steps && ok; ++i) {
-        const int st = i & 1, nx = (i + 1) & 1;
-        const bool more = i + 1 < steps;
-        if (kSB == 2 && more) {
-          if (!(ok = wait(&k_full[nx], ((i + 1) >> 1) & 1))) break;
-          qk(0, i + 1);
-          tc_commit(&s_full[nx]);
-          tc_commit(&k_empty[nx]);
-        }
-        if (!(ok = wait(&v_full[st], (i >> 1) & 1))) break;
-        for (int tile = 0; tile < kNQ; ++tile) {
-          if (!(ok = wait(&p_full[tile * kSB + (kSB == 2 ? st : 0)], kSB == 2 ? (i >> 1) & 1 : i & 1))) break;
-          tc_fence_after();
-          pv(tile, i);
-          tc_commit(more ? &o_done[tile] : &o_last[tile]);
-          if (tile == kNQ - 1) tc_commit(&v_empty[st]);
-          if (kSB == 1 && more) {
-            if (tile == 0 && !(ok = wait(&k_full[nx], ((i + 1) >> 1) & 1))) break;
-            qk(tile, i + 1);
-            tc_commit(&s_full[tile]);
-            if (tile == kNQ - 1) tc_commit(&k_empty[nx]);
+      while (w.u < u1 && ok) {
+        const int n = w.n;
+        if (lane == 0) {
+          for (int tile = 0; tile < kNQ && n && ok; ++tile) {
+            if (!(ok = wait(&q_full[tile], np & 1) && wait(&k_full[g0 & 1], (g0 >> 1) & 1))) break;
+            qk(tile, g0);
+            tc_commit(&s_full[tile * kSB + (kSB == 2 ? g0 & 1 : 0)]);
+            if (tile == kNQ - 1) tc_commit(&k_empty[g0 & 1]);
+          }
+          for (int i = 0; i < n && ok; ++i) {
+            const int g = g0 + i, st = g & 1, nx = st ^ 1;
+            const bool more = i + 1 < n;
+            if (kSB == 2 && more) {
+              if (!(ok = wait(&k_full[nx], ((g + 1) >> 1) & 1))) break;
+              qk(0, g + 1);
+              tc_commit(&s_full[nx]);
+              tc_commit(&k_empty[nx]);
+            }
+            if (!(ok = wait(&v_full[st], (g >> 1) & 1))) break;
+            for (int tile = 0; tile < kNQ; ++tile) {
+              if (!(ok = wait(&p_full[tile * kSB + (kSB == 2 ? st : 0)], kSB == 2 ? (g >> 1) & 1 : g & 1))) break;
+              tc_fence_after();
+              pv(tile, g, i > 0);
+              tc_commit(&o_done[tile]);
+              if (!more) tc_commit(&o_last[tile]);
+              if (tile == kNQ - 1) tc_commit(&v_empty[st]);
+              if (kSB == 1 && more) {
+                if (tile == 0 && !(ok = wait(&k_full[nx], ((g + 1) >> 1) & 1))) break;
+                qk(tile, g + 1);
+                tc_commit(&s_full[tile]);
+                if (tile == kNQ - 1) tc_commit(&k_empty[nx]);
+              }
+            }
           }
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (n) ++np;
+        g0 += n;
+        go_on();
       }
       // nothing may be in flight when TMEM is given back
-      tc_commit(fin);
-      volatile int no_abort = 0;
-      mbar_wait(fin, 0, &no_abort, status, kDevTimeoutDrain, 1000000000ull);
+      if (lane == 0) {
+        tc_commit(fin);
+        volatile int no_abort = 0;
+        mbar_wait(fin, 0, &no_abort, status, kDevTimeoutDrain, 1000000000ull);
+      }
     }
     __syncwarp();
   }
