@@ -131,7 +131,9 @@ long long workspace_size(int sms, int dim) {
   return most;
 }
 
-// From this many rows of a kv head on, the tcgen05 kernel
+// From this many query rows of a kv head on, the tcgen05 kernel.  32 heads, 8 kv heads, D = 128, both
+// sides in us (decode kernel, prompt kernel): 64 rows over 16000 tokens of one sequence 51 and 40, 128
+// rows 79 and 44; 32 sequences of 4000 tokens, 64 rows 161 and 148, 32 rows 97 and 168.
 constexpr int kPromptRows = 64;
 
 // Resident CTAs per SM, at most `most`, of a kernel with `smem` dynamic bytes on the current
@@ -174,17 +176,21 @@ int decode(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
 }
 
 template <int D, bool kCap>
-int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, int min_rows, void* workspace) {
+int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o, long long rows, int min_rows, void* workspace) {
   using Cfg = PromptCfg<D>;
   static std::atomic<int> known[64];
   if (resident(b2g_kv4_prompt_kernel<D, kCap>, Cfg::kThreads, Cfg::kSmem, 1, f.dev, known) < 1)
     return host_fail(B2G_ERR_CUDA, "the prompt kernel does not fit on the device");
+  const long long blocks = (rows + Cfg::kRows - 1) / Cfg::kRows;
+  if (blocks * f.c.heads * f.bt.seqs >= 4ll * f.sms && blocks <= 65535)
+    return launch(b2g_kv4_prompt_kernel<D, kCap>, dim3(f.c.heads, f.bt.seqs, static_cast<unsigned>(blocks)), Cfg::kThreads, Cfg::kSmem,
+                  f.st, f.c, f.bt, m, q, o, min_rows, nullptr, nullptr, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
   int4* desc = static_cast<int4*>(workspace);
   float* partial = reinterpret_cast<float*>(desc + f.sms);
   int rc = launch(b2g_kv4_prompt_kernel<D, kCap>, dim3(f.sms), Cfg::kThreads, Cfg::kSmem, f.st, f.c, f.bt, m, q, o, min_rows, partial,
                   desc, static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
   if (rc) return rc;
-  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, 16, true>, dim3(f.sms, Cfg::kRows / 16), 512, 0, f.st, f.bt, q, o, partial, desc);
+  return launch(b2g_kv4_join_kernel<D, Cfg::kRows, 16, true>, dim3(f.sms, 4), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
 template <int D>
@@ -268,13 +274,14 @@ int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, co
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
   const Kv4Out o{static_cast<__nv_bfloat16*>(out), out_row_stride, out_head_stride, lse};
   const long long rows = static_cast<long long>(std::max(1, batch->cu ? std::min(batch->max_new, batch->rows) : 1)) * qs.group;
-  // Prompts and single tokens in one batch: each kernel takes its own sequences.  Where the others are
-  // prompts too, judged by their average, one launch serves; what it serves is the same either way.
-  const bool mixed = f.bt.seqs > 1 && (batch->rows - batch->max_new) * static_cast<long long>(qs.group) < 4 * kPromptRows * (f.bt.seqs - 1);
+  // Prompts and single tokens in one batch: each kernel takes its own sequences.  Where the other
+  // sequences have 32 rows and more on average, one launch of the prompt kernel serves all sooner (75 us for
+  // both kernels, 39 for one: four sequences of 20 to 64 rows over 4000 tokens).
+  const bool mixed = f.bt.seqs > 1 && (batch->rows - batch->max_new) * static_cast<long long>(qs.group) < kPromptRows / 2 * (f.bt.seqs - 1ll);
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     const int limit = rows < kPromptRows ? INT_MAX : mixed ? static_cast<int>(kPromptRows) : 0;  // rows from which the prompt kernel takes a sequence
-    if (limit != INT_MAX) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, limit, workspace) : prompt<D, false>(f, m, qs, o, limit, workspace);
+    if (limit != INT_MAX) rc = m.softcap > 0.f ? prompt<D, true>(f, m, qs, o, rows, limit, workspace) : prompt<D, false>(f, m, qs, o, rows, limit, workspace);
     if (limit == 0 || rc) return;
     const long long here = std::min<long long>(rows, limit);
     if (here <= 4) rc = decode<D, 1, true>(f, m, qs, o, limit, workspace);

@@ -707,8 +707,8 @@ b2g_kv4_decode_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   griddep_launch_dependents();
 }
 
-// Joins the parts of an item that was cut: block (i, y) has kRB rows from kRB y on of the item that
-// CTA i began.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
+// Joins the parts of an item that was cut: blocks (i, *) have the item that CTA i began, kRB rows at a
+// time.  512 threads: 16 / kRB warps share a row's parts, eight in flight each.
 template <int D, int kRows, int kRB, bool kPlain>
 __global__ void __launch_bounds__(512)
 b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restrict__ partial, const int4* __restrict__ desc) {
@@ -724,7 +724,8 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
   const int blocks = (group_rows + kRows - 1) / kRows;
   const int h = d.z / blocks, r0 = (d.z - h * blocks) * kRows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int share = warp % kShare, r = blockIdx.y * kRB + warp / kShare;
+  const int share = warp % kShare;
+  for (int r = blockIdx.y * kRB + warp / kShare; r < kRows; r += gridDim.y * kRB) {
   float top = kNoMax, sum = 0.f, o[kE] = {};
   if (r0 + r < group_rows) {
 #pragma unroll 1
@@ -766,11 +767,14 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
       top = t;
     }
   }
+  if (kShare > 1) {
+    __syncthreads();  // the rows before these have been joined
 #pragma unroll
-  for (int e = 0; e < kE; e += 2) *reinterpret_cast<float2*>(&s_o[warp][e * 32 + 2 * lane]) = make_float2(o[e], o[e + 1]);
-  if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
-  __syncthreads();
-  if (share != 0 || r0 + r >= group_rows) return;
+    for (int e = 0; e < kE; e += 2) *reinterpret_cast<float2*>(&s_o[warp][e * 32 + 2 * lane]) = make_float2(o[e], o[e + 1]);
+    if (lane == 0) s_m[warp] = top, s_l[warp] = sum;
+    __syncthreads();
+  }
+  if (share != 0 || r0 + r >= group_rows) continue;
   float t = top;
 #pragma unroll
   for (int w = 1; w < kShare; ++w) t = fmaxf(t, s_m[warp + w]);
@@ -789,6 +793,7 @@ b2g_kv4_join_kernel(Kv4Batch bt, Kv4Queries q, Kv4Out out, const float* __restri
   const int head = h * q.group + (r0 + r) % q.group;
 #pragma unroll
   for (int e = 0; e < kE; e += 2) kv4_finish<kPlain>(out, row, head, q.heads, e * 16 + lane, make_float2(o[e], o[e + 1]), t, sum);
+  }
 }
 
 }  // namespace b2g

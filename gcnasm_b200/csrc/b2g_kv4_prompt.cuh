@@ -13,9 +13,14 @@
 // clock, its 2 x 128 x 128 exponentials 2048 at 16 a clock, decoding 32768 codes ~700 issue slots a
 // scheduler.  Hence two query tiles: while one's S is being exponentiated the other's products
 // run, and what a step decodes serves 256 rows.  D = 256 leaves TMEM for one query tile, whose S
-// has two buffers instead.  The items' steps, laid end to end, are cut evenly among one CTA on each
-// SM (whole waves of items left 15 % of the GPU idle at the end of 256 items, and most of it where
-// there are few); parts of a cut item are joined by a second kernel, as in the decode kernel.
+// has two buffers instead.
+//
+// Work: with four items (sequence, kv head, block of rows) or more for each SM, a CTA for each.  With
+// fewer, where whole waves leave SMs idle (15 % of the time of 256 items, nearly all of it for
+// one sequence's few rows over a long context), the items' steps are laid end to end and cut evenly
+// among one CTA on each SM; a second kernel joins the parts of a cut item, as for the decode kernel.
+// Measured: 656 items of 6 steps 160 us whole, 201 cut; 256 items of 121 steps 724 and 690; 8 of
+// 126 steps 370 and 49.
 //
 // Codes become bf16 as in the decode kernel (times 2^-64, exact), in the order 0 4 1 5 2 6 3 7 of
 // each eight channels: Q is stored in the same order, O's columns are put back when written.
@@ -49,8 +54,9 @@ struct PromptCfg {
   static constexpr int kOffBar = kOffV + 2 * kKBytes;
   static constexpr int kBars = 8 + 2 * kNQ * kSB + 3 * kNQ + 1;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;  // and room to align to 1024
-  // An item is cut into no less than this on average: a piece starts and ends in about two steps' time.
-  static constexpr int kMinSteps = 4;
+  // What an item takes besides its steps (Q, the first S, the output), in steps; and the least units of
+  // work for a CTA.
+  static constexpr int kItemUnits = 2, kMinUnits = 6;
   static constexpr uint32_t kColO = 256;  // S at column (tile * kSB + buffer) * kN, O here
 };
 
@@ -169,7 +175,7 @@ struct Kv4PromptPiece {
   int first, rows, len, group_rows;  // of the sequence
   int j0, steps;                     // of the item: its first step's number and how many it has
   int s0, n;                         // of the piece; n = 0 where no row of the item sees a token
-  long long u;                       // its first unit among all
+  long long u;                       // its first step's unit among all
 };
 
 template <int D>
@@ -193,12 +199,13 @@ __device__ __forceinline__ void kv4_prompt_item(Kv4PromptPiece& w, const Kv4Mask
   w.steps = max(0, (hi1 + PromptCfg<D>::kN - 1) / PromptCfg<D>::kN - w.j0);
 }
 
-// An item's units of work: its steps, one where it has none.
+// An item's units of work: kItemUnits that are no step, then its steps, one where it has none.  A
+// step belongs to the CTA whose range has its unit.
 template <int D>
 __device__ __forceinline__ int kv4_prompt_units(Kv4PromptPiece& w, int blk, const Kv4Mask& m, const Kv4Queries& q) {
   w.blk = blk;
   kv4_prompt_item<D>(w, m, q);
-  return max(1, w.steps);
+  return PromptCfg<D>::kItemUnits + max(1, w.steps);
 }
 
 __device__ __forceinline__ long long warp_sum(long long x) {
@@ -251,7 +258,8 @@ __device__ __forceinline__ long long kv4_prompt_scan(const Kv4Batch& bt, const K
   return sum;
 }
 
-// Sequences with at least min_rows query rows of a kv head.
+// Sequences with at least min_rows query rows of a kv head.  desc null: a grid of (kv heads,
+// sequences, blocks), whole items.
 template <int D, bool kCap>
 __global__ void __launch_bounds__(PromptCfg<D>::kThreads, 1)
 b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Out out, int min_rows, float* __restrict__ partial,
@@ -263,7 +271,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   __shared__ Kv4Found s_found;
   // each warp's piece: kept here, not in registers, which the loops over S need
   __shared__ Kv4PromptPiece s_piece[Cfg::kThreads / 32];
-  __shared__ long long s_u0, s_u1, s_total, s_ctas;
+  __shared__ long long s_u1, s_total, s_ctas;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
   uint64_t* k_full = bars;
@@ -282,10 +290,25 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   constexpr int kDecodeWarp = 4 * kNQ, kMmaWarp = kDecodeWarp + 4;
 
   griddep_wait();
-  // ---- work: all items' units end to end, cut evenly among the CTAs
   const int me = blockIdx.x;
-  if (threadIdx.x == 0) desc[me] = make_int4(0, 0, 0, 0);
-  {
+  if (!desc) {
+    // ---- work: a CTA for each item, those that see most first
+    Kv4PromptPiece w;
+    w.h = blockIdx.x;
+    w.b = blockIdx.y;
+    kv4_prompt_seq<D>(w, bt, q, c.page_log2, min_rows);
+    w.blk = w.blocks - 1 - static_cast<int>(blockIdx.z);
+    if (w.blk < 0) return;
+    kv4_prompt_item<D>(w, mask, q);
+    w.s0 = 0;
+    w.n = w.steps;
+    w.u = 0;
+    if (threadIdx.x == 0) s_u1 = max(1, w.steps);
+    if (lane == 0) s_piece[warp] = w;
+    __syncthreads();
+  } else {
+    // ---- work: all items' units end to end, cut evenly among the CTAs
+    if (threadIdx.x == 0) desc[me] = make_int4(0, 0, 0, 0);
     constexpr int kWarps = Cfg::kThreads / 32;
     const int per = (bt.seqs + kWarps - 1) / kWarps, b0 = min(warp * per, bt.seqs), b1 = min(b0 + per, bt.seqs);
     const long long mine = kv4_prompt_scan<D>(bt, mask, q, c.page_log2, min_rows, c.heads, b0, b1, 0, 0, nullptr);
@@ -296,11 +319,10 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       if (i < warp) before += s_scan[i];
       total += s_scan[i];
     }
-    const long long ctas = min(static_cast<long long>(gridDim.x), max(total / Cfg::kMinSteps, min(total, 1ll)));
+    const long long ctas = min(static_cast<long long>(gridDim.x), max(total / Cfg::kMinUnits, min(total, 1ll)));
     if (me >= ctas) return;
     const long long u = total * me / ctas;
     if (threadIdx.x == 0) {
-      s_u0 = u;
       s_u1 = total * (me + 1) / ctas;
       s_total = total;
       s_ctas = ctas;
@@ -310,7 +332,6 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       __syncwarp();
       Kv4PromptPiece w;
       w.b = s_found.b;
-      w.u = u;
       kv4_prompt_seq<D>(w, bt, q, c.page_log2, min_rows);
       w.h = static_cast<int>(s_found.unit / s_found.per_head);
       long long rest = s_found.unit - w.h * s_found.per_head;
@@ -318,7 +339,8 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
         const int units = base + lane < w.blocks ? kv4_prompt_units<D>(w, base + lane, mask, q) : 0;
         const long long upto = warp_scan(units, lane);
         if (upto - units <= rest && rest < upto) {
-          w.s0 = static_cast<int>(rest - (upto - units));
+          w.s0 = max(0, static_cast<int>(rest - (upto - units)) - Cfg::kItemUnits);
+          w.u = u + w.s0 + Cfg::kItemUnits - (rest - (upto - units));
           s_piece[0] = w;
         }
         const long long all = __shfl_sync(0xffffffffu, upto, 31);
@@ -328,7 +350,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     }
     __syncthreads();
     Kv4PromptPiece w = s_piece[0];
-    w.n = static_cast<int>(min(static_cast<long long>(w.steps - (w.steps ? w.s0 : 0)), s_u1 - u));
+    w.n = static_cast<int>(min(static_cast<long long>(w.steps - (w.steps ? w.s0 : 0)), s_u1 - w.u));
     __syncthreads();
     if (lane == 0) s_piece[warp] = w;
     __syncwarp();
@@ -338,7 +360,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
   // the next piece, where one is left
   auto go_on = [&]() {
     Kv4PromptPiece x = w;
-    x.u += max(1, x.n);
+    x.u += max(1, x.steps) - x.s0 + Cfg::kItemUnits;
     if (x.u < u1) {
       x.s0 = 0;
       if (++x.blk >= x.blocks) {
@@ -401,6 +423,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
     auto wait = [&](uint64_t* bar, uint32_t parity) {  // all lanes go on, or none: what follows is the warp's
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, kDevTimeoutEpilogue, timeout_ns)) != 0;
     };
+    int pieces = 0;  // the CTA's first goes to its first slot, a later one that is cut to its second
     while (w.u < u1 && ok) {
     const int r0 = w.blk * Cfg::kRows, r = r0 + tile * 128 + in_tile;
     const bool real = r < w.group_rows;
@@ -565,7 +588,7 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       tc_fence_after();
       const float f = l == 0.f ? 0.f : kTwo64 / l;
       uint8_t* dst = reinterpret_cast<uint8_t*>(out.out + row * out.row + head * out.head);
-      float* part = partial + (2ll * me + (w.u == s_u0 ? 0 : 1)) * (Cfg::kRows * (D + 2));
+      float* part = partial + (2ll * me + (pieces == 0 ? 0 : 1)) * (Cfg::kRows * (D + 2));
 #pragma unroll 1
       for (int col = 0; col < D; col += 32) {
         uint32_t x[32];
@@ -597,11 +620,12 @@ b2g_kv4_prompt_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, Kv4Ou
       if (!whole && w.s0 == 0 && threadIdx.x == 0) {
         // this CTA begins the item; the ones after it, up to the one with its last unit, go on
         const long long other = ((w.u + w.steps) * s_ctas - 1) / s_total;
-        desc[me] = make_int4(static_cast<int>(other) - me + 1, w.b, w.h * w.blocks + w.blk, w.u == s_u0 ? 0 : 1);
+        desc[me] = make_int4(static_cast<int>(other) - me + 1, w.b, w.h * w.blocks + w.blk, pieces == 0 ? 0 : 1);
       }
     }
     if (n) ++np;
     g0 += n;
+    ++pieces;
     go_on();
     }
   } else if (warp < kMmaWarp) {

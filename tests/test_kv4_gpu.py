@@ -188,6 +188,24 @@ def test_attention_groups_by_rows(kv4, group, new):
     attend(kv4, Case([new, 3 * new + 1], 2, 64, 16, seed=group + new), [new, new], 2 * group)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("news,lens,mask", [
+    ([1, 300, 1, 2, 1, 1], [700, 350, 1, 2, 900, 33], dict()),           # prompts and single tokens in one batch
+    ([70], [2500], dict()),                                              # few rows, many steps: cut across the GPU
+    ([65, 1, 1], [1500, 3000, 10], dict(window=700)),
+    ([40, 200], [2000, 200], dict(softcap=15.0)),
+    ([500, 0, 3], [500, 40, 1200], dict(causal=False)),
+])
+def test_attention_cut_and_mixed(kv4, D, news, lens, mask):
+    attend(kv4, Case(lens, 1, D, 64, seed=len(lens)), news, 2, **mask)
+
+
+def test_attention_many_items(kv4):
+    """More (sequence, head, block) items than the GPU takes at once."""
+    n = 50
+    attend(kv4, Case([100 + 3 * i for i in range(n)], 8, 64, 32, seed=3), [70 + i for i in range(n)], 16)
+
+
 @pytest.mark.parametrize("D", [64, 256])
 @pytest.mark.parametrize("new", [1, 6, 200])
 def test_attention_nothing_seen(kv4, D, new):
