@@ -3,8 +3,9 @@
 The product is the C ABI in ``include/b2g/gemm.h`` implemented by
 ``gcnasm_b200/_lib/libb2g.so`` (hand-written tcgen05 / TMA kernels).  This
 package binds it (``capi``), mirrors the reference's f4gemm host helpers
-(``f4gemm``) and offers torch-tensor wrappers (``ops``).
+(``f4gemm``) and offers torch-tensor wrappers (``ops``).  Beside the GEMMs stand
+the 4-bit key/value cache and its attention (``include/b2g/kv4.h``, ``kv4``).
 """
 from . import capi  # noqa: F401
 
-__all__ = ["capi", "f4gemm", "ops", "build"]
+__all__ = ["capi", "f4gemm", "kv4", "ops", "build"]

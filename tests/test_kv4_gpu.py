@@ -529,3 +529,42 @@ def test_refusals(kv4):
     out, _ = kv4.attention(q[:0], cache, table, lens, none)
     assert out.shape == (0, 4, 64)
     kv4.append(cache, kv[:0], kv[:0], table, lens, none)
+
+
+# ------------------------------------------------------------------ all together
+def test_layer_with_eviction(kv4):
+    """The demo's layer: prompts, then decode steps that thin the cache out.  Each step's output is that of
+    plain 64-bit attention over what the cache held, through the same projections."""
+    from gcnasm_b200 import kv4_demo, ops
+    torch.manual_seed(1)
+    dim, heads, kv_heads, D, budget = 256, 4, 2, 64, 48
+    layer = kv4_demo.KV4Attention(torch.randn(((heads + 2 * kv_heads) * D, dim), device="cuda") * dim ** -0.5,
+                                  torch.randn((dim, heads * D), device="cuda") * 0.06, heads, kv_heads, D, pages=64, page_size=16)
+    seen = []
+
+    class Spy:
+        def __getattr__(self, name):
+            return getattr(kv4, name)
+
+        def attention(self, q, cache, table, lens, cu=None, **k):
+            out, lse = kv4.attention(q, cache, table, lens, cu, **k)
+            n = lens.tolist()
+            c = cu.tolist() if cu is not None else list(range(len(n) + 1))
+            cpu = {x: getattr(cache, x).cpu() for x in ("k", "v", "k_scale", "v_scale")}
+            want = R.attention(q.cpu(), cpu, table.cpu(), n, c, 16, D ** -0.5)
+            within(out, want[0], want[2], "out")
+            within(lse, want[1], want[3], "lse")
+            seen.append(n)
+            return out, lse
+
+    real, kv4_demo.kv4 = kv4_demo.kv4, Spy()
+    try:
+        for y, lens in kv4_demo.generate(layer, [70, 20, 33], 40, dim, budget, every=8):
+            assert torch.isfinite(y).all() and y.shape[1] == dim
+    finally:
+        kv4_demo.kv4 = real
+    assert len(seen) == 41 and seen[0] == [70, 20, 33]
+    assert seen[1] == [49, 21, 34] and max(max(n) for n in seen[1:]) <= budget + 8
+    assert ops.device_status() == 0
+    # the weights that a sequence's tokens hold sum to at most one per query head and step seen
+    assert (layer.gathered >= 0).all()
