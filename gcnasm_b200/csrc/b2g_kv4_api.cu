@@ -12,6 +12,7 @@
 #include "b2g_host.h"
 #include "b2g_kv4.cuh"
 #include "b2g_kv4_decode.cuh"
+#include "b2g_kv4_gather.cuh"
 #include "b2g_kv4_prompt.cuh"
 #include "b2g_kv4_weights.cuh"
 
@@ -193,6 +194,21 @@ int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   return launch(b2g_kv4_join_kernel<D, Cfg::kRows, 16, true>, dim3(f.sms, 4), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
+// From this many query rows of a kv head on, the tcgen05 kernel
+constexpr int kGatherRows = 48;
+
+template <int D, bool kCap, bool kInOrder>
+int gather_many(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const float* lse, const float* w_in, float* w_out) {
+  using Cfg = GatherCfg<D>;
+  static std::atomic<int> few[64], many[64];
+  const bool is_few = f.bt.seqs <= 512;
+  const size_t smem = 1024 + ((Cfg::kFixed + 15) & ~15) + ((is_few ? 512 : 2048) + 1) * sizeof(long long);
+  const int n = resident(b2g_kv4_gather_kernel<D, kCap, kInOrder>, Cfg::kThreads, smem, 1, f.dev, is_few ? few : many);
+  if (n < 1) return host_fail(B2G_ERR_CUDA, "the gather kernel does not fit on the device");
+  return launch(b2g_kv4_gather_kernel<D, kCap, kInOrder>, dim3(f.sms), Cfg::kThreads, smem, f.st, f.c, f.bt, m, q, lse, w_in, w_out,
+                static_cast<uint64_t>(host_wait_timeout_ns()), f.status);
+}
+
 template <int D>
 int gather(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const float* lse, const float* w_in, float* w_out) {
   static std::atomic<int> few[64], many[64];
@@ -303,9 +319,13 @@ int b2g_kv4_weights(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, cons
     return host_fail(B2G_ERR_INVALID_ARG, "null or misaligned lse or weights");
   const Kv4Mask m{mask->scale, mask->softcap, mask->causal, mask->window};
   const Kv4Queries qs{static_cast<const __nv_bfloat16*>(q), q_row_stride, q_head_stride, heads, heads / f.c.heads};
+  const long long rows = static_cast<long long>(std::max(1, batch->cu ? std::min(batch->max_new, batch->rows) : 1)) * qs.group;
   by_dim(f.dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
-    rc = gather<D>(f, m, qs, lse, weights_in, weights_out);
+    // more sequences than the prefix sums have room for beside the tiles: the other kernel serves any
+    if (rows < kGatherRows || f.bt.seqs > 2048) rc = gather<D>(f, m, qs, lse, weights_in, weights_out);
+    else if (rows <= 128) rc = m.softcap > 0.f ? gather_many<D, true, true>(f, m, qs, lse, weights_in, weights_out) : gather_many<D, false, true>(f, m, qs, lse, weights_in, weights_out);
+    else rc = m.softcap > 0.f ? gather_many<D, true, false>(f, m, qs, lse, weights_in, weights_out) : gather_many<D, false, false>(f, m, qs, lse, weights_in, weights_out);
   });
   return rc;
 }

@@ -181,12 +181,12 @@ __device__ __forceinline__ Kv4Span kv4_span(const Kv4Batch& bt, const Kv4Mask& m
   return s;
 }
 
-// Units before each sequence, pre[0 .. seqs], by a CTA of 128 threads: each takes some
-// consecutive sequences.
-template <typename F>
+// Units before each sequence, pre[0 .. seqs], by a CTA of kThreads: each takes some consecutive
+// sequences.  warp_sum: a number for each warp.
+template <int kThreads = 128, typename F>
 __device__ __forceinline__ void kv4_scan(int seqs, long long* pre, long long* warp_sum, F&& units) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int per = (seqs + 127) / 128;
+  const int per = (seqs + kThreads - 1) / kThreads;
   long long sum = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;

@@ -1,0 +1,340 @@
+// b2g_kv4_gather.cuh -- the attention weight that each cached token gathers from many query rows,
+// on tcgen05 (few rows: b2g_kv4_weights.cuh).
+//
+//   S^T = K Q^T          tcgen05.mma, 128 tokens x 128 query rows, S^T in TMEM
+//   w_j += sum_i 2^(S_ji - lse_i)    one thread per token: its sum runs along its own TMEM row
+// With the tokens as the product's rows the column sums of the attention matrix need no exchange
+// between threads at all.  A unit of work is kNT tiles of 128 tokens of a kv head, whose K is
+// decoded once (bf16, times 2^-64, as for the prompt kernel) and meets the sequence's query rows
+// 128 at a time; where a CTA's next unit has the same rows, and no more than 128, Q stays.
+// Warps: one warpgroup of exponentials per token tile, four warps that decode K and stage Q, one
+// that issues the products; S^T has two buffers per tile, K two stages.
+//
+// What bounds it: the exponentials, 16 a clock on an SM: 2048 clocks for 256 tokens x 128 rows, where the
+// products take 1024 and decoding K ~700 issue slots a scheduler, once per unit.
+#pragma once
+
+#include "b2g_kv4_prompt.cuh"
+
+namespace b2g {
+
+template <int D>
+struct GatherCfg {
+  static constexpr int kNT = D == 256 ? 1 : 2;  // token tiles of a unit
+  static constexpr int kTokens = 128 * kNT;
+  static constexpr int kQS = D == 256 ? 1 : 2;  // stages of Q
+  static constexpr int kThreads = kNT * 128 + 256;
+  static constexpr int kTile = 128 * D * 2;     // bytes of 128 rows of K or Q
+  static constexpr int kOffQ = 2 * kNT * kTile;
+  static constexpr int kOffLse = kOffQ + kQS * kTile;   // per token tile: two buffers of 128
+  static constexpr int kOffBar = kOffLse + kNT * 2 * 128 * 4;
+  static constexpr int kBars = 4 + 2 * kQS + 4 * kNT + 1;
+  static constexpr int kFixed = kOffBar + kBars * 8 + 16;
+};
+
+struct Kv4GatherUnit {
+  int b, h, t0, first, rows, len;
+  int rb0, rb1;  // blocks of 128 query rows that see some of its tokens
+  bool keep;     // Q is the unit's before, still there
+};
+
+// kInOrder: a CTA's units are consecutive ones (of equal cost: no more than 128 rows); else every
+// gridDim.x-th, which spreads units of unequal cost.
+template <int D, bool kCap, bool kInOrder>
+__global__ void __launch_bounds__(GatherCfg<D>::kThreads, 1)
+b2g_kv4_gather_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, const float* __restrict__ lse, const float* w_in,
+                      float* w_out, uint64_t timeout_ns, int* status) {
+  using Cfg = GatherCfg<D>;
+  constexpr int kNT = Cfg::kNT, kQS = Cfg::kQS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_scan[Cfg::kThreads / 32];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBar);
+  uint64_t* k_full = bars;
+  uint64_t* k_empty = bars + 2;
+  uint64_t* s_full = bars + 4;                 // [tile][buffer]
+  uint64_t* s_empty = s_full + 2 * kNT;
+  uint64_t* q_full = s_empty + 2 * kNT;
+  uint64_t* q_empty = q_full + kQS;
+  uint64_t* fin = q_empty + kQS;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  long long* s_pre = reinterpret_cast<long long*>(smem + ((Cfg::kFixed + 15) & ~15));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kDecodeWarp = 4 * kNT, kMmaWarp = kDecodeWarp + 4;
+
+  griddep_wait();
+  kv4_scan<Cfg::kThreads>(bt.seqs, s_pre, s_scan, [&](int b) {
+    return static_cast<long long>((kv4_len(bt, b, c.page_log2) + Cfg::kTokens - 1) / Cfg::kTokens) * c.heads;
+  });
+  const long long total = s_pre[bt.seqs];
+  const long long u0 = kInOrder ? total * blockIdx.x / gridDim.x : blockIdx.x;
+  const long long u1 = kInOrder ? total * (blockIdx.x + 1) / gridDim.x : total, du = kInOrder ? 1 : gridDim.x;
+  if (u0 >= u1) return;
+  auto locate = [&](Kv4GatherUnit& x, long long u) {  // x: a unit before it, or b = -1
+    const int pb = x.b, ph = x.h, p0 = x.rb0, p1 = x.rb1;
+    x.b = max(x.b, 0);
+    while (u >= s_pre[x.b + 1]) ++x.b;
+    int end;
+    kv4_rows(bt, x.b, x.first, end);
+    x.rows = end - x.first;
+    x.len = kv4_len(bt, x.b, c.page_log2);
+    const int chunks = (x.len + Cfg::kTokens - 1) / Cfg::kTokens;
+    const long long in_seq = u - s_pre[x.b];
+    x.h = static_cast<int>(in_seq / chunks);
+    x.t0 = static_cast<int>(in_seq - static_cast<long long>(x.h) * chunks) * Cfg::kTokens;
+    // query tokens i (at len - rows + i) that see one of tokens t0 .. t1 - 1
+    const int t1 = min(x.t0 + Cfg::kTokens, x.len), shift = x.len - x.rows;
+    const long long lo = mask.causal ? max(0, x.t0 - shift) : 0;
+    const long long hi = mask.window > 0 ? min(static_cast<long long>(x.rows), static_cast<long long>(t1) - 1 + mask.window - shift) : x.rows;
+    x.rb0 = static_cast<int>(lo * q.group / 128);
+    x.rb1 = hi > lo ? static_cast<int>((hi * q.group + 127) / 128) : x.rb0;
+    x.keep = pb == x.b && ph == x.h && p0 == x.rb0 && p1 == x.rb1 && x.rb1 == x.rb0 + 1;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 128);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < kQS; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < 2 * kNT; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 128);
+    }
+    mbar_init(fin, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(tmem_holder);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  bool ok = true;
+  Kv4GatherUnit w;
+  w.b = -1;
+  w.h = w.rb0 = w.rb1 = -1;
+
+  if (warp < kDecodeWarp) {
+    // ---------------------------------------------------------------- exponentials: one thread per token
+    const int tile = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float* s_lse = reinterpret_cast<float*>(smem + Cfg::kOffLse) + tile * 256;
+    const float scale = mask.scale * kTwo64;
+    const float s_scale = kCap ? scale / mask.softcap : scale * kLog2e, cap2 = kCap ? mask.softcap * kLog2e : 0.f;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, kDevTimeoutEpilogue, timeout_ns)) != 0;
+    };
+    int g = 0;  // products of this tile so far
+    for (long long u = u0; u < u1 && ok; u += du) {
+      locate(w, u);
+      const int token = w.t0 + tile * 128 + row;
+      long long at = -1;
+      if (token < w.len) {
+        const int page = __ldg(bt.table + static_cast<long long>(w.b) * bt.width + (token >> c.page_log2));
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(c.pages))
+          at = ((static_cast<long long>(page) * c.heads + w.h) << c.page_log2) + (token & ((1 << c.page_log2) - 1));
+      }
+      const float before = at >= 0 ? w_in[at] : 0.f;
+      // rows [seen0, seen1) of the kv head see the token
+      const int shift = w.len - w.rows;
+      const long long seen0 = mask.causal ? static_cast<long long>(max(0, token - shift)) * q.group : 0;
+      const long long seen1 = (mask.window > 0 ? min(static_cast<long long>(w.rows), static_cast<long long>(token) + mask.window - shift) : w.rows) *
+                              static_cast<long long>(q.group);
+      float s0 = 0.f, s1 = 0.f;
+      for (int rb = w.rb0; rb < w.rb1 && ok; ++rb, ++g) {
+        const int buf = g & 1;
+        {  // -lse of the rows; -inf, a weight of zero, where there is no row or it sees nothing
+          const int n = rb * 128 + row;
+          float x = -INFINITY;
+          if (n < w.rows * q.group) {
+            const float v = __ldg(lse + static_cast<long long>(w.first + n / q.group) * q.heads + w.h * q.group + n % q.group);
+            if (v != -INFINITY) x = -v * kLog2e;
+          }
+          s_lse[buf * 128 + row] = x;
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(tile + 1) : "memory");
+        const bool masked = __any_sync(0xffffffffu, seen0 > rb * 128 || seen1 < rb * 128 + 128);
+        if (!(ok = wait(&s_full[tile * 2 + buf], (g >> 1) & 1))) break;
+        tc_fence_after();
+        const uint32_t s_at = tmem + lanes + (tile * 2 + buf) * 128;
+        auto chunk = [&](uint32_t (&x)[32], int col) {
+          uint32_t bits = 0xFFFFFFFFu;
+          if (masked) {
+            const long long from = rb * 128ll + col;
+            bits = kv4_bits(static_cast<int>(max(min(seen0 - from, 32ll), 0ll)), static_cast<int>(max(min(seen1 - from, 32ll), 0ll)));
+          }
+          if (kCap) {
+            float far = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) far = fmaxf(far, fabsf(__uint_as_float(x[e])));
+            if (__all_sync(0xffffffffu, far * fabsf(s_scale) < 0.4f)) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]);
+                mul2(y0, y1, s_scale, s_scale);
+                kv4_tanh_near2(y0, y1);
+                x[e] = __float_as_uint(y0), x[e + 1] = __float_as_uint(y1);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float y = __uint_as_float(x[e]) * s_scale;
+                x[e] = __float_as_uint(fabsf(y) < 0.4f ? kv4_tanh_near(y) : kv4_tanh_far(y));
+              }
+            }
+          }
+          const float k = kCap ? cap2 : s_scale;
+          const float4* ls = reinterpret_cast<const float4*>(s_lse + buf * 128 + col);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 l = ls[e >> 2];
+            float y0 = __uint_as_float(x[e]), y1 = __uint_as_float(x[e + 1]), y2 = __uint_as_float(x[e + 2]), y3 = __uint_as_float(x[e + 3]);
+            fma2(y0, y1, k, k, l.x, l.y);
+            fma2(y2, y3, k, k, l.z, l.w);
+            y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
+            if (masked) {
+              y0 = (bits >> e) & 1u ? y0 : 0.f;
+              y1 = (bits >> (e + 1)) & 1u ? y1 : 0.f;
+              y2 = (bits >> (e + 2)) & 1u ? y2 : 0.f;
+              y3 = (bits >> (e + 3)) & 1u ? y3 : 0.f;
+            }
+            add2(s0, s1, y0, y1);
+            add2(s0, s1, y2, y3);
+          }
+        };
+        uint32_t xa[32], xb[32];
+        tmem_ld_32x32b_x32(s_at, xa);
+#pragma unroll 1
+        for (int col = 0; col < 128; col += 64) {
+          tc_wait_ld();
+          tmem_ld_32x32b_x32(s_at + col + 32, xb);
+          chunk(xa, col);
+          tc_wait_ld();
+          if (col == 0) tmem_ld_32x32b_x32(s_at + 64, xa);
+          chunk(xb, col + 32);
+        }
+        tc_fence_before();
+        mbar_arrive(&s_empty[tile * 2 + buf]);
+      }
+      if (at >= 0 && ok) w_out[at] = before + (s0 + s1);
+    }
+  } else if (warp < kMmaWarp) {
+    // ---------------------------------------------------------------- K decoded, Q staged
+    constexpr int kWords = D / 8;  // a token's words of codes
+    const int tok = threadIdx.x - kDecodeWarp * 32;
+    int n = 0, gq = 0;  // units and blocks of Q so far
+    for (long long u = u0; u < u1 && ok; u += du) {
+      locate(w, u);
+      if (w.rb0 >= w.rb1) continue;
+      const int st = n & 1;
+      if (!mbar_wait(&k_empty[st], ((n >> 1) & 1) ^ 1, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
+#pragma unroll 1
+      for (int tile = 0; tile < kNT; ++tile) {
+        const int token = w.t0 + tile * 128 + tok;
+        long long at = -1;
+        if (token < w.len) at = kv4_token(c, bt.table + static_cast<long long>(w.b) * bt.width, w.h, token, status);
+        uint8_t* row = smem + (st * kNT + tile) * Cfg::kTile + tok * 128;
+#pragma unroll
+        for (int part = 0; part < (kWords + 15) / 16; ++part) {  // 16 words, four scales at a time
+          constexpr int kP = kWords < 16 ? kWords : 16;
+          uint4 x[kP / 4];
+          uint32_t scales = 0, even, odd;
+#pragma unroll
+          for (int i = 0; i < kP / 4; ++i) x[i] = at >= 0 ? *(reinterpret_cast<const uint4*>(c.k + at * (D / 2) + part * 64) + i) : make_uint4(0, 0, 0, 0);
+          if (at >= 0) {
+            if constexpr (D == 64) scales = *reinterpret_cast<const uint16_t*>(c.ks + at * 2);
+            else scales = *(reinterpret_cast<const uint32_t*>(c.ks + at * (D / 32)) + part);
+          }
+          kv4_scales_bf16<62>(scales, even, odd);
+#pragma unroll
+          for (int i = 0; i < kP / 4; ++i) {
+            const uint32_t f = __byte_perm(i & 1 ? odd : even, 0, i & 2 ? 0x3232 : 0x1010);
+            const uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int piece = part * 16 + i * 4 + e;
+              *reinterpret_cast<uint4*>(row + (piece >> 3) * (128 * 128) + (((piece & 7) ^ (tok & 7)) << 4)) =
+                  make_uint4(mul_bf16x2(kv4_raw<0>(word[e]), f), mul_bf16x2(kv4_raw<1>(word[e]), f), mul_bf16x2(kv4_raw<2>(word[e]), f),
+                             mul_bf16x2(kv4_raw<3>(word[e]), f));
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&k_full[st]);
+      ++n;
+      if (w.keep) continue;
+      for (int rb = w.rb0; rb < w.rb1; ++rb, ++gq) {
+        const int qs = gq % kQS;
+        if (!mbar_wait(&q_empty[qs], ((gq / kQS) & 1) ^ 1, abort_flag, status, kDevTimeoutProducer, timeout_ns)) { ok = false; break; }
+        const int r = rb * 128 + tok;
+        uint8_t* dst = smem + Cfg::kOffQ + qs * Cfg::kTile + tok * 128;
+        const bool real = r < w.rows * q.group;
+        const uint4* src = reinterpret_cast<const uint4*>(q.q + (w.first + r / q.group) * q.q_row + (w.h * q.group + r % q.group) * q.q_head);
+#pragma unroll 8
+        for (int i = 0; i < D / 8; ++i) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (real) x = __ldg(src + i);
+          *reinterpret_cast<uint4*>(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (tok & 7)) << 4)) =
+              make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[qs]);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t kId = idesc_bf16(128, 128, 0);
+    int n = 0, g = 0, gq = 0;  // units, products of a tile and blocks of Q so far
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, status, kDevTimeoutMma, timeout_ns); };
+    locate(w, u0);
+    for (long long u = u0; u < u1 && ok; u += du) {
+      Kv4GatherUnit next = w;
+      if (u + du < u1) locate(next, u + du);
+      if (w.rb0 < w.rb1 && lane == 0) {
+        const int st = n & 1;
+        ok = wait(&k_full[st], (n >> 1) & 1);
+        for (int rb = w.rb0; rb < w.rb1 && ok; ++rb, ++g) {
+          const int qi = w.keep ? gq - 1 : gq, qs = qi % kQS;
+          if (!w.keep) {
+            if (!(ok = wait(&q_full[qs], (qi / kQS) & 1))) break;
+            ++gq;
+          }
+          for (int tile = 0; tile < kNT; ++tile) {
+            if (!(ok = wait(&s_empty[tile * 2 + (g & 1)], ((g >> 1) & 1) ^ 1))) break;
+            tc_fence_after();
+            const uint32_t a = smem_u32(smem + (st * kNT + tile) * Cfg::kTile), bq = smem_u32(smem + Cfg::kOffQ + qs * Cfg::kTile);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_bf16_ss(tmem + (tile * 2 + (g & 1)) * 128, desc_kmajor_sw128(a + (k >> 2) * (128 * 128) + (k & 3) * 32),
+                          desc_kmajor_sw128(bq + (k >> 2) * (128 * 128) + (k & 3) * 32), kId, k > 0);
+            tc_commit(&s_full[tile * 2 + (g & 1)]);
+          }
+          if (ok && !(u + du < u1 && next.keep)) tc_commit(&q_empty[qs]);
+        }
+        if (ok) tc_commit(&k_empty[st]);
+        ++n;
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      w = next;
+    }
+    // nothing may be in flight when TMEM is given back
+    if (lane == 0) {
+      tc_commit(fin);
+      volatile int no_abort = 0;
+      mbar_wait(fin, 0, &no_abort, status, kDevTimeoutDrain, 1000000000ull);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc<512>(tmem);
+}
+
+}  // namespace b2g

@@ -74,9 +74,9 @@ b2g_kv4_weights_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, cons
     x.rows = end - x.first;
     x.len = kv4_len(bt, x.b, c.page_log2);
     const int chunks = (x.len + kWeightTokens - 1) / kWeightTokens;
-    const int in_seq = static_cast<int>(u - s_pre[x.b]);
-    x.h = in_seq / chunks;
-    x.tok0 = (in_seq - x.h * chunks) * kWeightTokens;
+    const long long in_seq = u - s_pre[x.b];
+    x.h = static_cast<int>(in_seq / chunks);
+    x.tok0 = static_cast<int>(in_seq - static_cast<long long>(x.h) * chunks) * kWeightTokens;
     int lo, hi, unused;
     kv4_visible(mask, x.len - x.rows, x.len, lo, unused);
     kv4_visible(mask, x.len - 1, x.len, unused, hi);
