@@ -194,7 +194,10 @@ int prompt(const Call& f, const Kv4Mask& m, const Kv4Queries& q, const Kv4Out& o
   return launch(b2g_kv4_join_kernel<D, Cfg::kRows, 16, true>, dim3(f.sms, 4), 512, 0, f.st, f.bt, q, o, partial, desc);
 }
 
-// From this many query rows of a kv head on, the tcgen05 kernel
+// From this many query rows of a kv head on, the tcgen05 kernel.  32 heads, 8 kv heads, D = 128, both
+// sides in us (weights kernel, tcgen05 kernel): one sequence of 32000 tokens, 32 rows 35 and 35, 64 rows
+// 51 and 37; 32 sequences of 4000 tokens, 32 rows 86 and 107, 64 rows 125 and 108.  64 rows of 8
+// sequences of 8000 tokens: D = 64 61 and 52, D = 256 133 and 92.
 constexpr int kGatherRows = 48;
 
 template <int D, bool kCap, bool kInOrder>

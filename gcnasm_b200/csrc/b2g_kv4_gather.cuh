@@ -10,8 +10,13 @@
 // Warps: one warpgroup of exponentials per token tile, four warps that decode K and stage Q, one
 // that issues the products; S^T has two buffers per tile, K two stages.
 //
-// What bounds it: the exponentials, 16 a clock on an SM: 2048 clocks for 256 tokens x 128 rows, where the
-// products take 1024 and decoding K ~700 issue slots a scheduler, once per unit.
+// What bounds it: latency.  Its exponentials take 2048 clocks for 256 tokens x 128 rows at 16 a clock on
+// an SM, the products 1024, decoding K ~700 issue slots a scheduler.  Three sequences of 32000 tokens, 128
+// rows of each of 8 kv heads, D = 128: 59 us, or ~7000 clocks a unit -- 2700 of sums, the rest the steps
+// before and after them in each role: pages, lse, codes, the way through the barriers.  Without the
+// exponentials it takes 55, without reading K 51.  Measured and slower, for the registers that they take:
+// codes fetched one half ahead 60 to 65, two threads a token 81; two CTAs with one tile each 55 here, but
+// 242 instead of 160 with 1024 rows of each kv head, as Q is staged twice as often.
 #pragma once
 
 #include "b2g_kv4_prompt.cuh"
@@ -81,14 +86,15 @@ b2g_kv4_gather_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, const
     x.len = kv4_len(bt, x.b, c.page_log2);
     const int chunks = (x.len + Cfg::kTokens - 1) / Cfg::kTokens;
     const long long in_seq = u - s_pre[x.b];
-    x.h = static_cast<int>(in_seq / chunks);
+    // every warp comes here for every unit: in 64 bits throughout it took 2 us of 59
+    x.h = in_seq < 0x7fffffffll ? static_cast<int>(in_seq) / chunks : static_cast<int>(in_seq / chunks);
     x.t0 = static_cast<int>(in_seq - static_cast<long long>(x.h) * chunks) * Cfg::kTokens;
     // query tokens i (at len - rows + i) that see one of tokens t0 .. t1 - 1
     const int t1 = min(x.t0 + Cfg::kTokens, x.len), shift = x.len - x.rows;
-    const long long lo = mask.causal ? max(0, x.t0 - shift) : 0;
-    const long long hi = mask.window > 0 ? min(static_cast<long long>(x.rows), static_cast<long long>(t1) - 1 + mask.window - shift) : x.rows;
-    x.rb0 = static_cast<int>(lo * q.group / 128);
-    x.rb1 = hi > lo ? static_cast<int>((hi * q.group + 127) / 128) : x.rb0;
+    const int lo = mask.causal ? max(0, x.t0 - shift) : 0;
+    const int hi = mask.window > 0 ? static_cast<int>(min(static_cast<long long>(x.rows), static_cast<long long>(t1) - 1 + mask.window - shift)) : x.rows;
+    x.rb0 = hi > lo ? lo * q.group / 128 : 0;
+    x.rb1 = hi > lo ? (hi * q.group + 127) / 128 : 0;
     x.keep = pb == x.b && ph == x.h && p0 == x.rb0 && p1 == x.rb1 && x.rb1 == x.rb0 + 1;
   };
 
@@ -126,11 +132,12 @@ b2g_kv4_gather_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, const
     float* s_lse = reinterpret_cast<float*>(smem + Cfg::kOffLse) + tile * 256;
     const float scale = mask.scale * kTwo64;
     const float s_scale = kCap ? scale / mask.softcap : scale * kLog2e, cap2 = kCap ? mask.softcap * kLog2e : 0.f;
+    // a wait that gave up leaves out the sums, but its warp still meets the tile's others at their barrier
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, kDevTimeoutEpilogue, timeout_ns)) != 0;
     };
     int g = 0;  // products of this tile so far
-    for (long long u = u0; u < u1 && ok; u += du) {
+    for (long long u = u0; u < u1; u += du) {
       locate(w, u);
       const int token = w.t0 + tile * 128 + row;
       long long at = -1;
@@ -142,11 +149,10 @@ b2g_kv4_gather_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, const
       const float before = at >= 0 ? w_in[at] : 0.f;
       // rows [seen0, seen1) of the kv head see the token
       const int shift = w.len - w.rows;
-      const long long seen0 = mask.causal ? static_cast<long long>(max(0, token - shift)) * q.group : 0;
-      const long long seen1 = (mask.window > 0 ? min(static_cast<long long>(w.rows), static_cast<long long>(token) + mask.window - shift) : w.rows) *
-                              static_cast<long long>(q.group);
+      const int seen0 = (mask.causal ? min(max(0, token - shift), w.rows) : 0) * q.group;
+      const int seen1 = (mask.window > 0 ? max(static_cast<int>(min(static_cast<long long>(w.rows), static_cast<long long>(token) + mask.window - shift)), 0) : w.rows) * q.group;
       float s0 = 0.f, s1 = 0.f;
-      for (int rb = w.rb0; rb < w.rb1 && ok; ++rb, ++g) {
+      for (int rb = w.rb0; rb < w.rb1; ++rb, ++g) {
         const int buf = g & 1;
         {  // -lse of the rows; -inf, a weight of zero, where there is no row or it sees nothing
           const int n = rb * 128 + row;
@@ -159,14 +165,14 @@ b2g_kv4_gather_kernel(Kv4Cache c, Kv4Batch bt, Kv4Mask mask, Kv4Queries q, const
         }
         asm volatile("bar.sync %0, 128;" ::"r"(tile + 1) : "memory");
         const bool masked = __any_sync(0xffffffffu, seen0 > rb * 128 || seen1 < rb * 128 + 128);
-        if (!(ok = wait(&s_full[tile * 2 + buf], (g >> 1) & 1))) break;
+        if (!ok || !(ok = wait(&s_full[tile * 2 + buf], (g >> 1) & 1))) continue;
         tc_fence_after();
         const uint32_t s_at = tmem + lanes + (tile * 2 + buf) * 128;
         auto chunk = [&](uint32_t (&x)[32], int col) {
           uint32_t bits = 0xFFFFFFFFu;
           if (masked) {
-            const long long from = rb * 128ll + col;
-            bits = kv4_bits(static_cast<int>(max(min(seen0 - from, 32ll), 0ll)), static_cast<int>(max(min(seen1 - from, 32ll), 0ll)));
+            const int from = rb * 128 + col;
+            bits = kv4_bits(seen0 - from, seen1 - from);
           }
           if (kCap) {
             float far = 0.f;

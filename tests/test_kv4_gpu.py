@@ -386,6 +386,11 @@ def test_in_a_graph(kv4):
     (2, 1, [32, 40], [32, 300], dict(window=20)),
     (1, 16, [64, 5], [500, 64], dict(causal=False)),
     (1, 3, [150, 4], [100, 2], dict()),
+    (2, 4, [16, 20, 1], [900, 1500, 5], dict()),
+    (1, 8, [16], [2000], dict(window=300)),
+    (2, 2, [40, 0, 40], [600, 300, 50], dict(softcap=8.0)),
+    (1, 6, [70, 90], [400, 3000], dict(window=1000, softcap=25.0)),
+    (3, 2, [30, 30], [520, 1030], dict(causal=False, window=200)),
 ])
 def test_weights(kv4, D, hk, group, news, lens, mask):
     c = Case(lens, hk, D, 32, seed=7)
