@@ -26,6 +26,13 @@
 // cut evenly: the (sequence, kv head, row block) items, laid end to end in units of 128
 // tokens, are divided among as many CTAs as fit on the GPU.  An item cut across CTAs leaves
 // partial results that a second kernel joins in a fixed order.
+//
+// Measured, one row of 48 ragged sequences of up to 8192 tokens, 32 heads, 8 kv heads, D = 128 (269 MB
+// read): 89 us, 3.0 TB/s, schedulers issuing 64 % of the time.  Issue slots bind it, 447 instructions for 16
+// tokens: loads alone take 55 us, all but V's conversion 81, all but the second terms' products 88,
+// all but K's conversion 96 (of 97 then); 16 warps on an SM instead of 12 change nothing.  Two sequences
+// of 131072 tokens with 16 rows a kv head: 68 us, 122 MB -- there the products take 30 % of the
+// tensor pipe at 8 warps on an SM.
 #pragma once
 
 #include "b2g_kv4.cuh"
@@ -261,7 +268,8 @@ __device__ __forceinline__ void kv4_stage_q(const Kv4Queries& q, int first, int 
 }
 
 // kTwin: up to four rows, each twice in a tile of eight -- the second time with the weights'
-// second terms, which then take no product of their own (decode_batch: 8 us of 97).
+// second terms, which then take no product of their own (8 us of 97: 48 ragged sequences of up to 8192
+// tokens, 32 heads, 8 kv heads, D = 128).
 template <int D, int NT, bool kTwin>
 struct DecodeCfg {
   static_assert(!kTwin || NT == 1, "one tile of eight");

@@ -12,9 +12,9 @@
 //
 // What bounds it: latency.  Its exponentials take 2048 clocks for 256 tokens x 128 rows at 16 a clock on
 // an SM, the products 1024, decoding K ~700 issue slots a scheduler.  Three sequences of 32000 tokens, 128
-// rows of each of 8 kv heads, D = 128: 59 us, or ~7000 clocks a unit -- 2700 of sums, the rest the steps
+// rows of each of 8 kv heads, D = 128: 57 us, or ~7000 clocks a unit -- 2700 of sums, the rest the steps
 // before and after them in each role: pages, lse, codes, the way through the barriers.  Without the
-// exponentials it takes 55, without reading K 51.  Measured and slower, for the registers that they take:
+// exponentials it takes 54, without reading K 49.  Measured and slower, for the registers that they take:
 // codes fetched one half ahead 60 to 65, two threads a token 81; two CTAs with one tile each 55 here, but
 // 242 instead of 160 with 1024 rows of each kv head, as Q is staged twice as often.
 #pragma once

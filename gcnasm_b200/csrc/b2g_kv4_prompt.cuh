@@ -14,6 +14,11 @@
 // scheduler.  Hence two query tiles: while one's S is being exponentiated the other's products
 // run, and what a step decodes serves 256 rows.  D = 256 leaves TMEM for one query tile, whose S
 // has two buffers instead.
+// Measured, 2048 query tokens at the end of 16500, 32 heads, 8 kv heads, D = 128: 700 to 730 us, 711 to 742 TFLOP/s of Q K^T
+// and P V counted once; the tensor pipe is busy 51 % of the time (P's second terms are half as much
+// again), the rest is the softmax warps, whose step of 128 tokens takes longer than its products.  Five
+// prompts of up to 1900 tokens, 24 heads, D = 64, capped scores: 173 us, tensor pipe 14 %: tanh, exponential
+// and conversion of each score on 128 threads a tile bind it.
 //
 // Work: with four items (sequence, kv head, block of rows) or more for each SM, a CTA for each.  With
 // fewer, where whole waves leave SMs idle (15 % of the time of 256 items, nearly all of it for

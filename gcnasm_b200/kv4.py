@@ -6,7 +6,8 @@ scale byte per 32 channels, the formats of :func:`ops.mxfp4_gemm`'s operands -- 
 slot ``j % page_size``; ``lens[b]`` counts its cached tokens, this step's among them.  The rows
 ``cu[b]:cu[b + 1]`` of q, k and v are its last tokens, in order; without ``cu`` each sequence
 has one row.  ``table``, ``lens`` and ``cu`` are int32 on the GPU, so that a decode loop never
-waits for it; ``max_new`` / ``max_q`` tell the host how many rows a sequence has at most.
+waits for it; ``max_new`` / ``max_q`` tell the host how many rows a sequence has at most (rows past
+that may be left unwritten).
 
 PyTorch supplies memory and streams; the computation runs in ``libb2g.so``
 (``include/b2g/kv4.h`` has the exact semantics).

@@ -15,7 +15,9 @@
  * the kernels bound them: a length is cut to the table's capacity, a row range to the
  * rows given, and a page number outside [0, pages) makes its tokens absent (not written,
  * not attended to, read as zeros) and sets the device status word to B2G_DEV_BAD_PAGE
- * (b2g_device_status).
+ * (b2g_device_status).  The kernels for many query rows wait on their own barriers with the
+ * limit of b2g_set_wait_timeout_ms, after which they end and the status word says which wait
+ * gave up, as for the GEMMs; what such a call wrote is not to be used.
  */
 #ifndef B2G_KV4_H
 #define B2G_KV4_H
@@ -52,7 +54,8 @@ typedef struct b2g_kv4_cache {
 /* The sequences of one call.  lens[b] counts sequence b's cached tokens, this step's
  * among them; its rows of q / k / v are cu[b] .. cu[b + 1] - 1 (cu[0] = 0, ascending)
  * and stand for its last tokens, in order.  cu = NULL: one row for each sequence
- * (rows = seqs).  max_new: an upper bound of a sequence's rows (host side).
+ * (rows = seqs).  max_new: an upper bound of a sequence's rows, by which the host chooses
+ * kernels and grids: rows of a sequence past it may be left unwritten.
  * seqs 1 .. 8192. */
 typedef struct b2g_kv4_batch {
     const int* table; /* [seqs][table_width] page numbers */
@@ -95,7 +98,8 @@ B2G_API int b2g_kv4_read(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch,
  * contiguous.  A query that sees no token gives out = 0, lse = -inf.  q, out: bf16,
  * element (row, head, channel) at row * *_row_stride + head * *_head_stride + channel,
  * bases and strides whole 16 bytes.  heads a multiple of kv_heads.
- * workspace: b2g_kv4_workspace_bytes(head_dim) bytes, 16-byte aligned, of any content.
+ * workspace: b2g_kv4_workspace_bytes(head_dim) bytes (20 to 40 MB on 148 SMs), 16-byte
+ * aligned, of any content.
  * Calls that overlap on the GPU need a workspace each. */
 B2G_API int b2g_kv4_attention(const b2g_kv4_cache* cache, const b2g_kv4_batch* batch, const b2g_kv4_mask* mask,
                               const void* q, long long q_row_stride, long long q_head_stride, int heads, void* out,
