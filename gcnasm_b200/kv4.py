@@ -68,6 +68,15 @@ def _raw_stream(stream, device: torch.device) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _as_current(stream, device: torch.device):
+    """A context with `stream` as the current one: what a call allocates belongs to the stream that it
+    runs on, and takes no memory that work on another is not yet done with."""
+    if not isinstance(stream, torch.cuda.Stream):
+        raw = _raw_stream(stream, device)
+        stream = torch.cuda.ExternalStream(raw, device) if raw else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
+
+
 def _ints(t: torch.Tensor, name: str, size: int) -> int:
     if t.dtype is not _I32 or not t.is_cuda or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of one dimension")
@@ -137,11 +146,14 @@ def read(cache: KV4Cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Te
          stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 (k, v) ``[rows, kv_heads, head_dim]``: rows ``cu[b]:cu[b + 1]`` hold sequence b's tokens
     ``start[b]``, ``start[b] + 1``, ... as the cache has them."""
+    if stream is not None:
+        with _as_current(stream, cache.k.device):
+            return read(cache, table, start, cu, rows)
     b = _batch(table, None, cu, rows, None)
     sp = _ints(start, "start", b.seqs)
     shape = (rows, cache.kv_heads, cache.head_dim)
     k, v = cache.k.new_empty(shape, dtype=_BF16), cache.k.new_empty(shape, dtype=_BF16)
-    capi.check(capi.lib().b2g_kv4_read(cache._args, b, sp, k.data_ptr(), v.data_ptr(), _raw_stream(stream, k.device)),
+    capi.check(capi.lib().b2g_kv4_read(cache._args, b, sp, k.data_ptr(), v.data_ptr(), _raw_stream(None, k.device)),
                "b2g_kv4_read")
     return k, v
 
@@ -175,6 +187,9 @@ def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch
     (``causal``) and j > p - window (``window`` > 0); scores are ``scale * q . k`` (default
     head_dim ** -0.5), capped as ``softcap * tanh(s / softcap)``.  lse fp32 ``[rows, heads]`` is the
     logarithm of the sum of exp(scores); a query that sees nothing gives out 0 and lse -inf."""
+    if stream is not None:
+        with _as_current(stream, q.device):
+            return attention(q, cache, table, lens, cu, max_q, scale, causal, window, softcap, out, ws)
     rows, heads, q_row, q_head = _heads(q, "q", cache)
     if q.dtype is not _BF16:
         raise ValueError(f"q must be bf16, not {q.dtype}")
@@ -187,7 +202,7 @@ def attention(q: torch.Tensor, cache: KV4Cache, table: torch.Tensor, lens: torch
         if out.dtype is not _BF16 or o_rows != rows or o_heads != heads:
             raise ValueError("out must be bf16 of q's shape")
     lse = q.new_empty((rows, heads), dtype=_F32)
-    st = _raw_stream(stream, q.device)
+    st = _raw_stream(None, q.device)
     if ws is None:
         ws = _workspace(cache, st)
     mask = capi.Kv4Mask(cache.head_dim ** -0.5 if scale is None else scale, softcap, causal, window)
@@ -225,6 +240,9 @@ def evict(cache: KV4Cache, gathered: torch.Tensor, table: torch.Tensor, lens: to
     to the pages of ``out_table`` (default: in place, to the first pages of ``table``), their gathered
     weights with them.  kept: int32 ``[seqs, kv_heads, budget]``, the numbers they had, then -1;
     ``out_lens`` may be ``lens``."""
+    if stream is not None:
+        with _as_current(stream, lens.device):
+            return evict(cache, gathered, table, lens, budget, sink, recent, out_table, out_lens)
     b = _batch(table, lens, None, table.shape[0], None)
     op, out_seqs, out_width = (b.table, b.seqs, b.table_width) if out_table is None else _table(out_table, "out_table")
     if out_seqs != b.seqs:
@@ -234,5 +252,5 @@ def evict(cache: KV4Cache, gathered: torch.Tensor, table: torch.Tensor, lens: to
     kept = lens.new_empty((b.seqs, cache.kv_heads, max(budget, 0)))
     capi.check(capi.lib().b2g_kv4_evict(cache._args, b, _weights_array(gathered, "gathered", cache), budget, sink, recent, op,
                                         out_width, kept.data_ptr(), _ints(out_lens, "out_lens", b.seqs),
-                                        _raw_stream(stream, lens.device)), "b2g_kv4_evict")
+                                        _raw_stream(None, lens.device)), "b2g_kv4_evict")
     return kept, out_lens

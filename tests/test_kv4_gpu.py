@@ -255,6 +255,29 @@ def test_attention_strides_and_streams(kv4, new):
     assert (buf == 3.0).all()
 
 
+@pytest.mark.parametrize("raw", [False, True])
+def test_results_belong_to_the_stream_of_the_call(kv4, raw):
+    """Memory that unfinished work of the current stream still writes is not given to a call on another."""
+    c = Case([400, 222], 2, 128, 64)
+    cu, table, lens, dcu = c.ints([3, 3])
+    q = torch.randn((6, 8, 128), generator=c.g).to(torch.bfloat16).cuda()
+    cache, start = c.gpu(kv4), torch.zeros(2, dtype=torch.int32, device="cuda")
+    want = (*kv4.attention(q, cache, table, lens, dcu, max_q=3), *kv4.read(cache, table, start, dcu, 6))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy = [torch.empty_like(t) for t in want for _ in range(4)]
+    torch.cuda._sleep(20_000_000)
+    for t in busy:
+        t.fill_(3.0)
+    del busy, t
+    stream = side.cuda_stream if raw else side
+    got = (*kv4.attention(q, cache, table, lens, dcu, max_q=3, stream=stream),
+           *kv4.read(cache, table, start, dcu, 6, stream=stream))
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("new", [1, 3, 90])
 def test_attention_is_repeatable(kv4, new):
     """Bit for bit the same in every run, with other calls between: sums are in a fixed order."""
